@@ -564,6 +564,101 @@ int vox_attention_gqa_step_noalloc(const float* d_query, const float* d_keys,
                                    const float* d_values, const vox_attention_shape* shape,
                                    float* d_out, void* stream);
 
+/* ---- paged key/value cache (no counterpart in the reference) --------------------- */
+/* Many sequences of different lengths in one pool of pages.  Every pointer in
+ * these calls is DEVICE memory the caller owns (on `device` of the cache);
+ * the calls are asynchronous on `stream` (a cudaStream_t, 0 = default
+ * stream), allocate nothing, keep nothing between calls, may be captured into
+ * a graph, and leave the calling thread's current device as it was.  All
+ * tensors of a call have the cache's dtype: VOX_DT_F32, VOX_DT_F16 or
+ * VOX_DT_BF16.  Strides are in elements.
+ *
+ * One layer's pool.  Element d of the key of slot s of page p, kv head h is
+ * keys[p * page_stride + h * head_stride + s * slot_stride + d]; values alike.
+ * The three strides may all be 0: packed [n_pages, n_kv_heads, page_size,
+ * head_dim].  page_size is a power of two in 1..1024, head_dim even and at
+ * most 256. */
+typedef struct vox_paged_cache {
+    int device;
+    int dtype; /* vox_tensor_dtype */
+    void* keys;
+    void* values;
+    size_t n_pages, page_size, n_kv_heads, head_dim;
+    size_t page_stride, head_stride, slot_stride;
+} vox_paged_cache;
+/* A ragged batch.  Sequence s has the tokens q_start[s] .. q_start[s+1] of the
+ * call and kv_len[s] tokens in the cache, the call's own included, so its i-th
+ * token has index kv_len[s] - q_len + i in the cache; index t lives in slot
+ * t % page_size of page page_table[s * table_stride + t / page_size].
+ * first_pos (nullable: 0) is the absolute position of index 0.  n_tokens,
+ * max_q_len and max_kv_len are the host's bounds on what the device arrays
+ * hold, so that a captured graph serves every step within them.  Tokens
+ * behind the last sequence are left alone.
+ *
+ * The device arrays are checked by the kernels.  A sequence whose lengths are
+ * negative, out of order or beyond the bounds or its table row is skipped
+ * (nothing of it is read or written) and VOX_PAGED_BAD_LENGTH set in *status;
+ * a page id outside the pool, where a visible or new token needs it, reads as
+ * zeros, is not written, and sets VOX_PAGED_BAD_PAGE.  *status (nullable)
+ * receives bits by atomic or; the caller clears it. */
+typedef struct vox_paged_batch {
+    size_t n_seqs, n_tokens, max_q_len, max_kv_len;
+    size_t table_width, table_stride; /* columns of the table, elements from row to row */
+    const int32_t* q_start;           /* [n_seqs + 1], from 0 on */
+    const int32_t* kv_len;            /* [n_seqs] */
+    const int32_t* page_table;        /* [n_seqs, table_width] */
+    const int64_t* first_pos;         /* [n_seqs], nullable */
+    uint32_t* status;                 /* nullable */
+} vox_paged_batch;
+#define VOX_PAGED_BAD_LENGTH 1u
+#define VOX_PAGED_BAD_PAGE 2u
+/* [n_tokens, heads, head_dim] with a unit last stride; both strides 0 = packed. */
+typedef struct vox_rows {
+    void* ptr;
+    size_t token_stride, head_stride;
+} vox_rows;
+/* Keys and values of the batch's tokens into their slots, the keys rotated as
+ * vox_rope_interleaved_inplace does at position first_pos + index (angles
+ * exact modulo a turn at any position), and, where q is not NULL, the queries
+ * rotated from q to q_out (which may be q itself).  rope_theta 0: no rotation;
+ * otherwise >= 1.  A token before the cache's first slot (kv_len < q_len) is
+ * not stored.  Two tokens of a call must not have the same slot. */
+int vox_paged_append_rope(const vox_paged_cache* cache, const vox_paged_batch* batch, const vox_rows* k_new,
+                          const vox_rows* v_new, float rope_theta, size_t n_heads, const vox_rows* q,
+                          const vox_rows* q_out, void* stream);
+/* Causal grouped-query attention over the cache: the token with index p sees
+ * index j <= p if j < n_sinks, or j > p - sliding_window, or sliding_window is
+ * 0 (as in vox_attention_gqa_step).  A token that sees nothing gets zeros.
+ * Keys and values that a token does not see do not affect it, whatever they
+ * hold; page ids that no token needs are not looked at.  scale 0 =
+ * 1/sqrt(head_dim).  f16 and bf16 tensors are multiplied as they are and
+ * accumulated in f32.  `workspace` is scratch memory of the size that
+ * vox_paged_attention_workspace gives (it may be 0), 256-byte aligned; calls
+ * that can overlap on the GPU need one each. */
+int vox_paged_attention_workspace(const vox_paged_cache* cache, const vox_paged_batch* batch, size_t n_heads,
+                                  size_t sliding_window, size_t n_sinks, size_t* bytes);
+int vox_paged_attention(const vox_paged_cache* cache, const vox_paged_batch* batch, const vox_rows* q,
+                        size_t n_heads, size_t sliding_window, size_t n_sinks, float scale, const vox_rows* out,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* The same for a batch whose sequences all begin with one shared prefix,
+ * which is read and multiplied once for all of them: *prefix_len tokens (a
+ * device int32, at most max_prefix_len) in the pages prefix_pages
+ * [n_prefix_pages].  The batch's table, kv_len and bounds are those of the
+ * sequences' own tokens behind the prefix; a token's index, for the window
+ * and the sinks, is *prefix_len + its index among its sequence's own. */
+typedef struct vox_paged_prefix {
+    const int32_t* pages;
+    const int32_t* len;
+    size_t n_pages, max_len;
+} vox_paged_prefix;
+int vox_paged_prefix_attention_workspace(const vox_paged_cache* cache, const vox_paged_batch* batch,
+                                         const vox_paged_prefix* prefix, size_t n_heads, size_t sliding_window,
+                                         size_t n_sinks, size_t* bytes);
+int vox_paged_prefix_attention(const vox_paged_cache* cache, const vox_paged_batch* batch,
+                               const vox_paged_prefix* prefix, const vox_rows* q, size_t n_heads,
+                               size_t sliding_window, size_t n_sinks, float scale, const vox_rows* out,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

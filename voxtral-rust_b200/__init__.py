@@ -122,6 +122,36 @@ class PipelineConfig(C.Structure):
                 ("prompt", StreamPromptConfig)]
 
 
+class PagedCacheDesc(C.Structure):
+    """vox_paged_cache: one layer's pool of pages (device memory of the caller)."""
+
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("keys", VP), ("values", VP), ("n_pages", SZ),
+                ("page_size", SZ), ("n_kv_heads", SZ), ("head_dim", SZ), ("page_stride", SZ), ("head_stride", SZ),
+                ("slot_stride", SZ)]
+
+
+class PagedBatchDesc(C.Structure):
+    """vox_paged_batch: a ragged batch over the pages."""
+
+    _fields_ = [("n_seqs", SZ), ("n_tokens", SZ), ("max_q_len", SZ), ("max_kv_len", SZ), ("table_width", SZ),
+                ("table_stride", SZ), ("q_start", VP), ("kv_len", VP), ("page_table", VP), ("first_pos", VP),
+                ("status", VP)]
+
+
+class PagedPrefixDesc(C.Structure):
+    """vox_paged_prefix: the pages that every sequence of a batch begins with."""
+
+    _fields_ = [("pages", VP), ("len", VP), ("n_pages", SZ), ("max_len", SZ)]
+
+
+class Rows(C.Structure):
+    """vox_rows: [n_tokens, heads, head_dim] with a unit last stride."""
+
+    _fields_ = [("ptr", VP), ("token_stride", SZ), ("head_stride", SZ)]
+
+
+PAGED_BAD_LENGTH, PAGED_BAD_PAGE = 1, 2
+
 _lib = None
 
 _SIGS = {
@@ -196,6 +226,11 @@ _SIGS = {
     "vox_silu_inplace": ([VP, F32P, SZ], C.c_int),
     "vox_softmax_inplace": ([VP, F32P, SZ], C.c_int),
     "vox_attention_gqa_step_noalloc": ([VP, VP, VP, C.POINTER(AttentionShape), VP, VP], C.c_int),
+    "vox_paged_append_rope": ([VP, VP, VP, VP, C.c_float, SZ, VP, VP, VP], C.c_int),
+    "vox_paged_attention_workspace": ([VP, VP, SZ, SZ, SZ, C.POINTER(SZ)], C.c_int),
+    "vox_paged_attention": ([VP, VP, VP, SZ, SZ, SZ, C.c_float, VP, VP, SZ, VP], C.c_int),
+    "vox_paged_prefix_attention_workspace": ([VP, VP, VP, SZ, SZ, SZ, C.POINTER(SZ)], C.c_int),
+    "vox_paged_prefix_attention": ([VP, VP, VP, VP, SZ, SZ, SZ, C.c_float, VP, VP, SZ, VP], C.c_int),
     "vox_weights_open": ([C.c_char_p, C.POINTER(VP)], C.c_int),
     "vox_weights_close": ([VP], None),
     "vox_weights_count": ([VP], SZ),
@@ -1092,3 +1127,207 @@ def softmax_inplace(ctx: Context, x):
     d = _f32(x).copy()
     _check(lib().vox_softmax_inplace(ctx.h, _p(d), d.size))
     return d
+
+
+# ---------------------------------------------------------------------------
+# Paged key/value cache (torch CUDA tensors; no counterpart in the reference)
+# ---------------------------------------------------------------------------
+# These calls take torch CUDA tensors, run on the current stream of the
+# tensors' device and return without synchronising.  Scratch memory and new
+# outputs come from torch's allocator, so calls on several streams and in
+# several captured graphs do not share any.
+
+_paged_dtypes = None
+
+
+def _paged_dtype(t, name):
+    global _paged_dtypes
+    if _paged_dtypes is None:
+        import torch
+        _paged_dtypes = {torch.float32: DTYPES.index("F32"), torch.float16: DTYPES.index("F16"),
+                         torch.bfloat16: DTYPES.index("BF16")}
+    if t.dtype not in _paged_dtypes:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16")
+    return _paged_dtypes[t.dtype]
+
+
+def _paged_stream(device):
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class PagedKvCache:
+    """One layer's pool of pages: k_pages and v_pages are CUDA tensors
+    [n_pages, n_kv_heads, page_size, head_dim] of one dtype (float32, float16
+    or bfloat16) with the same strides, the last one 1 (a transposed
+    [n_pages, page_size, n_kv_heads, head_dim] pool, or the halves of one
+    tensor, are fine).  The tensors stay the caller's."""
+
+    def __init__(self, k_pages, v_pages):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+            raise ValueError("k_pages and v_pages must be [n_pages, n_kv_heads, page_size, head_dim], "
+                             "with the same shape and strides")
+        if k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device or not k_pages.is_cuda:
+            raise ValueError("k_pages and v_pages must have one dtype and be on one CUDA device")
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = (int(n) for n in k_pages.shape)
+        page, head, slot, unit = k_pages.stride()
+        if unit != 1 and self.head_dim > 1:
+            raise ValueError("the head dimension of the pages must be contiguous")
+        # the stride of a dimension of size 1 says nothing
+        slot = slot if self.page_size > 1 else self.head_dim
+        head = head if self.n_kv_heads > 1 else max(slot, self.head_dim)
+        page = page if self.n_pages > 1 else max(head, slot, self.head_dim)
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.dtype, self.device = k_pages.dtype, k_pages.device
+        self.desc = PagedCacheDesc(k_pages.device.index, _paged_dtype(k_pages, "k_pages"), k_pages.data_ptr(),
+                                   v_pages.data_ptr(), self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
+                                   page, head, slot)
+        self._ref = C.addressof(self.desc)
+
+
+class PagedBatch:
+    """A ragged batch over a paged cache: sequence s has the tokens
+    q_start[s] .. q_start[s+1] of a call and kv_len[s] cached tokens, the
+    call's own included, in the pages page_table[s, :].
+
+    q_start int32 [n_seqs + 1], kv_len int32 [n_seqs], page_table int32
+    [n_seqs, pages], first_pos (absolute position of each sequence's index 0;
+    default 0) int64 [n_seqs] and status (VOX_PAGED_* bits) int32 [1] are CUDA
+    tensors, read when the kernels run: a captured graph follows them within
+    the host's bounds n_tokens, max_q_len and max_kv_len (default: the table's
+    capacity)."""
+
+    def __init__(self, q_start, kv_len, page_table, n_tokens, max_q_len, max_kv_len=None, first_pos=None, status=None):
+        import torch
+        i32 = torch.int32
+        n = int(kv_len.shape[0]) if kv_len.dim() == 1 else -1
+        if n < 0 or q_start.dim() != 1 or q_start.shape[0] != n + 1 or page_table.dim() != 2 or \
+                page_table.shape[0] != n:
+            raise ValueError("q_start must be [n_seqs + 1], kv_len [n_seqs] and page_table [n_seqs, pages]")
+        if q_start.dtype != i32 or kv_len.dtype != i32 or page_table.dtype != i32:
+            raise ValueError("q_start, kv_len and page_table must be int32")
+        if first_pos is not None and (first_pos.dtype != torch.int64 or tuple(first_pos.shape) != (n,)):
+            raise ValueError("first_pos must be int64 [n_seqs]")
+        if status is not None and (status.dtype != i32 or status.numel() != 1):
+            raise ValueError("status must be int32 [1]")
+        for t in (q_start, kv_len, page_table, first_pos, status):
+            if t is not None and (not t.is_cuda or t.device != kv_len.device):
+                raise ValueError("the batch's tensors must be on one CUDA device")
+            if t is not None and t is not page_table and not t.is_contiguous():
+                raise ValueError("q_start, kv_len, first_pos and status must be contiguous")
+        if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+            raise ValueError("the rows of page_table must be contiguous")
+        self.device, self.n_seqs, self.n_tokens = kv_len.device, n, int(n_tokens)
+        self._keep = (q_start, kv_len, page_table, first_pos, status)
+        width = int(page_table.shape[1])
+        self._auto_max_kv = max_kv_len is None
+        self.desc = PagedBatchDesc(n, self.n_tokens, int(max_q_len), 0 if max_kv_len is None else int(max_kv_len),
+                                   width, int(page_table.stride(0)) if n > 1 else width, q_start.data_ptr(),
+                                   kv_len.data_ptr(), page_table.data_ptr(),
+                                   first_pos.data_ptr() if first_pos is not None else None,
+                                   status.data_ptr() if status is not None else None)
+        self._ref = C.addressof(self.desc)
+        self._workspace_bytes = {}
+
+    def _for(self, cache):
+        if self.device != cache.device:
+            raise ValueError("the batch and the cache must be on one device")
+        if self._auto_max_kv:
+            self.desc.max_kv_len = self.desc.table_width * cache.page_size
+        return self._ref
+
+
+def _paged_rows(t, name, batch, heads, cache):
+    if t.dim() != 3 or t.shape[0] != batch.n_tokens or t.shape[1] != heads or t.shape[2] != cache.head_dim:
+        raise ValueError(f"{name} must be [{batch.n_tokens}, {heads}, {cache.head_dim}]")
+    if t.dtype != cache.dtype or t.device != cache.device:
+        raise ValueError(f"{name} must have the cache's dtype and device")
+    token, head, unit = t.stride()
+    if unit != 1 and t.shape[2] > 1:
+        raise ValueError(f"the head dimension of {name} must be contiguous")
+    if token == 0 and head == 0 and t.shape[0] * t.shape[1] > 1:
+        raise ValueError(f"{name} must not be one row expanded over tokens and heads")
+    return Rows(t.data_ptr(), token, head)
+
+
+def paged_append_rope(cache: PagedKvCache, batch: PagedBatch, k_new, v_new, rope_theta, q=None, q_out=None):
+    """Keys and values [n_tokens, n_kv_heads, head_dim] of the batch's tokens
+    into their slots, the keys rotated (rope_interleaved_inplace's pairs) to
+    their positions; queries [n_tokens, n_heads, head_dim], if given, rotated
+    into q_out (a new tensor by default; q itself is fine), which is returned.
+    rope_theta 0: no rotation (vox_paged_append_rope)."""
+    ref = batch._for(cache)
+    k = _paged_rows(k_new, "k_new", batch, cache.n_kv_heads, cache)
+    v = _paged_rows(v_new, "v_new", batch, cache.n_kv_heads, cache)
+    heads, qr, qo = 0, None, None
+    if q is not None:
+        import torch
+        heads = int(q.shape[1]) if q.dim() == 3 else 0
+        qr = _paged_rows(q, "q", batch, heads, cache)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        qo = _paged_rows(q_out, "q_out", batch, heads, cache)
+    _check(lib().vox_paged_append_rope(cache._ref, ref, C.addressof(k), C.addressof(v), rope_theta, heads,
+                                       C.addressof(qr) if qr is not None else None,
+                                       C.addressof(qo) if qo is not None else None, _paged_stream(cache.device)))
+    return q_out
+
+
+def _paged_attention(cache, batch, prefix, q, sliding_window, n_sinks, scale, out):
+    import torch
+    ref = batch._for(cache)
+    heads = int(q.shape[1]) if q.dim() == 3 else 0
+    qr = _paged_rows(q, "q", batch, heads, cache)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    orow = _paged_rows(out, "out", batch, heads, cache)
+    L = lib()
+    # the scratch size follows from the host's bounds alone
+    what = (heads, sliding_window, n_sinks, None if prefix is None else prefix.max_len, batch.desc.max_kv_len,
+            cache.dtype, cache.n_kv_heads, cache.head_dim, cache.page_size)
+    n = batch._workspace_bytes.get(what)
+    if n is None:
+        got = SZ()
+        if prefix is None:
+            _check(L.vox_paged_attention_workspace(cache._ref, ref, heads, sliding_window, n_sinks, C.byref(got)))
+        else:
+            _check(L.vox_paged_prefix_attention_workspace(cache._ref, ref, C.addressof(prefix), heads, sliding_window,
+                                                          n_sinks, C.byref(got)))
+        n = batch._workspace_bytes[what] = got.value
+    ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
+    wp = ws.data_ptr() if n else None
+    if prefix is None:
+        _check(L.vox_paged_attention(cache._ref, ref, C.addressof(qr), heads, sliding_window, n_sinks, scale,
+                                     C.addressof(orow), wp, n, _paged_stream(cache.device)))
+    else:
+        _check(L.vox_paged_prefix_attention(cache._ref, ref, C.addressof(prefix), C.addressof(qr), heads,
+                                            sliding_window, n_sinks, scale, C.addressof(orow), wp, n,
+                                            _paged_stream(cache.device)))
+    return out
+
+
+def paged_attention(cache: PagedKvCache, batch: PagedBatch, q, sliding_window=0, n_sinks=0, scale=0.0, out=None):
+    """Causal grouped-query attention of the batch's queries [n_tokens,
+    n_heads, head_dim] over the cache: a token sees the last sliding_window
+    tokens (0: all), its own included, and the first n_sinks of its sequence.
+    scale 0 = 1/sqrt(head_dim).  Returns out [n_tokens, n_heads, head_dim];
+    rows behind the last sequence are left as they were (vox_paged_attention)."""
+    return _paged_attention(cache, batch, None, q, sliding_window, n_sinks, scale, out)
+
+
+def paged_prefix_attention(cache: PagedKvCache, batch: PagedBatch, prefix_pages, prefix_len, max_prefix_len, q,
+                           sliding_window=0, n_sinks=0, scale=0.0, out=None):
+    """paged_attention for a batch whose sequences all begin with one shared
+    prefix, read once for all of them: prefix_len (CUDA int32 [1], at most
+    max_prefix_len) tokens in the pages prefix_pages (CUDA int32 [pages]).  The
+    batch describes the sequences' own tokens behind it; sliding_window and
+    n_sinks count from the prefix's first token (vox_paged_prefix_attention)."""
+    import torch
+    if prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or not prefix_pages.is_contiguous() or \
+            prefix_len.dtype != torch.int32 or prefix_len.numel() != 1:
+        raise ValueError("prefix_pages must be contiguous int32 [pages] and prefix_len int32 [1]")
+    if prefix_pages.device != cache.device or prefix_len.device != cache.device:
+        raise ValueError("the prefix and the cache must be on one device")
+    prefix = PagedPrefixDesc(prefix_pages.data_ptr(), prefix_len.data_ptr(), int(prefix_pages.shape[0]),
+                             int(max_prefix_len))
+    return _paged_attention(cache, batch, prefix, q, sliding_window, n_sinks, scale, out)

@@ -1,0 +1,344 @@
+// vox_paged.cpp -- host side of the paged key/value cache: checks the
+// arguments, plans the launch from the host's bounds (never from device data)
+// and launches.  Nothing is allocated and nothing is kept between calls.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/vox_decoder.h"
+#include "vox_host.h"
+#include "vox_paged.h"
+
+using namespace vox;
+
+namespace {
+
+#define TRY(expr)                      \
+    do {                               \
+        int rc_ = (expr);              \
+        if (rc_ != VOX_OK) return rc_; \
+    } while (0)
+
+// Makes the cache's device current for the call.
+class DeviceGuard {
+  public:
+    int enter(int device) {
+        // An error left by earlier work is the caller's: reported, not mistaken for one of this call.
+        if (cudaPeekAtLastError() != cudaSuccess)
+            return report_errorf(VOX_ERR_CUDA, "an earlier CUDA error is pending on this thread; nothing was launched");
+        if (cudaGetDevice(&before_) != cudaSuccess) return no_device(device);
+        if (before_ != device) {
+            if (cudaSetDevice(device) != cudaSuccess) return no_device(device);
+            switched_ = true;
+        }
+        return VOX_OK;
+    }
+    ~DeviceGuard() {
+        if (switched_) cudaSetDevice(before_);
+    }
+
+  private:
+    static int no_device(int device) {
+        const char* why = cudaGetErrorString(cudaGetLastError());
+        return report_errorf(VOX_ERR_CUDA, "cannot use device %d: %s", device, why);
+    }
+    int before_ = 0;
+    bool switched_ = false;
+};
+
+int launched(cudaError_t e, const char* what) {
+    if (e == cudaSuccess) return VOX_OK;
+    (void)cudaGetLastError();
+    return report_errorf(VOX_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+}
+
+int shift_of(size_t n) {
+    int s = 0;
+    while ((size_t(1) << s) < n) ++s;
+    return s;
+}
+
+size_t type_size(PagedType t) { return t == PagedType::F32 ? 4 : 2; }
+
+struct Checked {
+    PagedType type;
+    int64_t page_stride, head_stride, slot_stride;
+    int page_shift;
+};
+
+constexpr size_t kMaxCount = INT32_MAX / 4;  // tokens, sequences, pages
+
+int check_cache(const vox_paged_cache* c, Checked* out) {
+    if (!c) return report_errorf(VOX_ERR_INVALID_ARG, "null cache");
+    switch (c->dtype) {
+        case VOX_DT_F32: out->type = PagedType::F32; break;
+        case VOX_DT_F16: out->type = PagedType::F16; break;
+        case VOX_DT_BF16: out->type = PagedType::BF16; break;
+        default: return report_errorf(VOX_ERR_UNSUPPORTED, "cache dtype must be f32, f16 or bf16");
+    }
+    if (!c->keys || !c->values) return report_errorf(VOX_ERR_INVALID_ARG, "null keys or values");
+    if (c->n_pages == 0 || c->n_pages > kMaxCount || c->n_kv_heads == 0 || c->n_kv_heads > 4096)
+        return report_errorf(VOX_ERR_INVALID_ARG, "n_pages and n_kv_heads (at most 4096) must be > 0");
+    if (c->page_size == 0 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return report_errorf(VOX_ERR_UNSUPPORTED, "page_size must be a power of two in 1..1024");
+    if (c->head_dim == 0 || c->head_dim % 2 || c->head_dim > (size_t)kPagedMaxHeadDim)
+        return report_errorf(VOX_ERR_UNSUPPORTED, "head_dim must be even and at most %d", kPagedMaxHeadDim);
+    out->page_shift = shift_of(c->page_size);
+    if (!c->page_stride && !c->head_stride && !c->slot_stride) {
+        out->slot_stride = c->head_dim;
+        out->head_stride = c->head_dim * c->page_size;
+        out->page_stride = out->head_stride * c->n_kv_heads;
+    } else {
+        if (c->slot_stride < c->head_dim || c->head_stride < c->head_dim ||
+            (c->n_pages > 1 && c->page_stride < c->head_dim) ||
+            std::max({c->page_stride, c->head_stride, c->slot_stride}) > (size_t(1) << 40))
+            return report_errorf(VOX_ERR_SHAPE, "cache strides must be at least head_dim");
+        out->page_stride = c->page_stride;
+        out->head_stride = c->head_stride;
+        out->slot_stride = c->slot_stride;
+    }
+    const size_t mis = type_size(out->type) - 1;
+    if (((uintptr_t)c->keys | (uintptr_t)c->values) & mis)
+        return report_errorf(VOX_ERR_INVALID_ARG, "keys or values are not aligned to their type");
+    return VOX_OK;
+}
+
+int check_batch(const vox_paged_cache* c, const vox_paged_batch* b) {
+    if (!b) return report_errorf(VOX_ERR_INVALID_ARG, "null batch");
+    if (b->n_seqs > kMaxCount || b->n_tokens > kMaxCount || b->max_kv_len > kMaxCount || b->table_width > kMaxCount ||
+        b->table_stride > (size_t(1) << 40))
+        return report_errorf(VOX_ERR_UNSUPPORTED, "batch sizes must be at most %d", (int)kMaxCount);
+    if (b->n_seqs == 0 || b->n_tokens == 0) return VOX_OK;
+    if (!b->q_start || !b->kv_len || (b->table_width && !b->page_table))
+        return report_errorf(VOX_ERR_INVALID_ARG, "null q_start, kv_len or page_table");
+    if (b->max_q_len == 0 || b->max_q_len > b->n_tokens)
+        return report_errorf(VOX_ERR_SHAPE, "max_q_len must be in 1..n_tokens");
+    if (b->max_kv_len > b->table_width * c->page_size)
+        return report_errorf(VOX_ERR_SHAPE, "max_kv_len needs more pages than the table has columns");
+    if (b->n_seqs > 1 && b->table_stride < b->table_width)
+        return report_errorf(VOX_ERR_SHAPE, "table_stride must be at least table_width");
+    return VOX_OK;
+}
+
+// [n_tokens, heads, head_dim] rows: strides, alignment to the type.  Rows that
+// are written must not overlap.
+int check_rows(const vox_rows* r, const char* name, size_t tokens, size_t heads, size_t hd, PagedType t, bool written,
+               int64_t* ts, int64_t* hs) {
+    if (!r || !r->ptr) return report_errorf(VOX_ERR_INVALID_ARG, "null %s", name);
+    if ((uintptr_t)r->ptr & (type_size(t) - 1))
+        return report_errorf(VOX_ERR_INVALID_ARG, "%s is not aligned to its type", name);
+    if (!r->token_stride && !r->head_stride) {
+        *ts = (int64_t)(heads * hd);
+        *hs = (int64_t)hd;
+        return VOX_OK;
+    }
+    if (std::max(r->token_stride, r->head_stride) > (size_t(1) << 40))
+        return report_errorf(VOX_ERR_SHAPE, "%s strides out of range", name);
+    if (written && ((tokens > 1 && r->token_stride < hd) || (heads > 1 && r->head_stride < hd)))
+        return report_errorf(VOX_ERR_SHAPE, "%s strides must be at least head_dim", name);
+    *ts = (int64_t)r->token_stride;
+    *hs = (int64_t)r->head_stride;
+    return VOX_OK;
+}
+
+bool aligned16(const void* p, PagedType t, std::initializer_list<int64_t> strides) {
+    if ((uintptr_t)p & 15) return false;
+    for (int64_t s : strides)
+        if ((s * (int64_t)type_size(t)) & 15) return false;
+    return true;
+}
+
+template <class A>
+void fill_common(A& a, const vox_paged_cache* c, const Checked& k, const vox_paged_batch* b) {
+    a.page_stride = k.page_stride;
+    a.head_stride = k.head_stride;
+    a.slot_stride = k.slot_stride;
+    a.n_pages = (int)c->n_pages;
+    a.page_shift = k.page_shift;
+    a.n_kv = (int)c->n_kv_heads;
+    a.hd = (int)c->head_dim;
+    a.n_seqs = (int)b->n_seqs;
+    a.n_tokens = (int)b->n_tokens;
+    a.max_q = (int)b->max_q_len;
+    a.max_kv = (int)b->max_kv_len;
+    a.table_width = (int)b->table_width;
+    a.table_stride = (int64_t)b->table_stride;
+    a.q_start = b->q_start;
+    a.kv_len = b->kv_len;
+    a.table = b->page_table;
+    a.status = b->status;
+}
+
+// What a call launches, from the host's bounds.
+struct AttnPlan {
+    int splits = 1;         // parts of the sequences' own keys
+    int prefix_splits = 0;  // parts of the shared prefix's
+    bool partial = false;   // through the workspace
+    size_t ml_bytes = 0, bytes = 0;
+};
+
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+AttnPlan plan_attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_paged_prefix* p, size_t n_heads,
+                        size_t window, size_t sinks) {
+    AttnPlan plan;
+    (void)window;
+    (void)sinks;
+    plan.splits = 1;
+    plan.prefix_splits = p ? 1 : 0;
+    plan.partial = plan.splits + plan.prefix_splits > 1;
+    if (plan.partial) {
+        const size_t rows = (size_t)(plan.splits + plan.prefix_splits) * b->n_tokens * n_heads;
+        plan.ml_bytes = round256(rows * sizeof(float2));
+        plan.bytes = plan.ml_bytes + rows * c->head_dim * sizeof(float);
+    }
+    return plan;
+}
+
+int check_attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_paged_prefix* p, size_t n_heads,
+                    Checked* k) {
+    TRY(check_cache(c, k));
+    TRY(check_batch(c, b));
+    if (n_heads == 0 || n_heads > 65536 || n_heads % c->n_kv_heads)
+        return report_errorf(VOX_ERR_INVALID_ARG, "n_heads must be > 0 and divisible by n_kv_heads");
+    if (p) {
+        if (!p->len || (p->n_pages && !p->pages)) return report_errorf(VOX_ERR_INVALID_ARG, "null prefix pages or length");
+        if (p->n_pages > kMaxCount || p->max_len > kMaxCount)
+            return report_errorf(VOX_ERR_UNSUPPORTED, "prefix sizes must be at most %d", (int)kMaxCount);
+        if (p->max_len > p->n_pages * c->page_size)
+            return report_errorf(VOX_ERR_SHAPE, "max_len needs more pages than the prefix has");
+    }
+    return VOX_OK;
+}
+
+int attention_workspace(const vox_paged_cache* c, const vox_paged_batch* b, const vox_paged_prefix* p, size_t n_heads,
+                        size_t window, size_t sinks, size_t* bytes) {
+    if (!bytes) return report_errorf(VOX_ERR_INVALID_ARG, "null bytes");
+    Checked k;
+    TRY(check_attention(c, b, p, n_heads, &k));
+    *bytes = b->n_seqs && b->n_tokens ? plan_attention(c, b, p, n_heads, window, sinks).bytes : 0;
+    return VOX_OK;
+}
+
+int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_paged_prefix* p, const vox_rows* q,
+              size_t n_heads, size_t window, size_t sinks, float scale, const vox_rows* out, void* ws, size_t ws_bytes,
+              void* stream) {
+    Checked k;
+    TRY(check_attention(c, b, p, n_heads, &k));
+    if (!(scale >= 0.f) || !std::isfinite(scale)) return report_errorf(VOX_ERR_INVALID_ARG, "scale must be finite and >= 0");
+    if (b->n_seqs == 0 || b->n_tokens == 0) return VOX_OK;
+    PagedAttnArgs a{};
+    fill_common(a, c, k, b);
+    a.k = c->keys;
+    a.v = c->values;
+    TRY(check_rows(q, "q", b->n_tokens, n_heads, c->head_dim, k.type, false, &a.q_ts, &a.q_hs));
+    TRY(check_rows(out, "out", b->n_tokens, n_heads, c->head_dim, k.type, true, &a.o_ts, &a.o_hs));
+    a.q = q->ptr;
+    a.out = out->ptr;
+    a.n_heads = (int)n_heads;
+    a.group = (int)(n_heads / c->n_kv_heads);
+    a.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
+    a.window = window >= kMaxCount * 2 ? 0 : (int)window;
+    a.sinks = (int)std::min(sinks, kMaxCount * 2);
+    if (p) {
+        a.pfx_pages = p->pages;
+        a.pfx_len = p->len;
+        a.pfx_n_pages = (int)p->n_pages;
+        a.pfx_max = (int)p->max_len;
+    }
+    const AttnPlan plan = plan_attention(c, b, p, n_heads, window, sinks);
+    if (plan.partial) {
+        if (!ws || ws_bytes < plan.bytes || ((uintptr_t)ws & 255))
+            return report_errorf(VOX_ERR_INVALID_ARG, "workspace must be %zu bytes, 256-byte aligned", plan.bytes);
+        a.part_ml = static_cast<float2*>(ws);
+        a.part_o = reinterpret_cast<float*>(static_cast<char*>(ws) + plan.ml_bytes);
+    }
+    DeviceGuard dev;
+    TRY(dev.enter(c->device));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p) {
+        PagedAttnArgs shared = a;
+        shared.in_prefix = 1;
+        shared.splits = plan.prefix_splits;
+        TRY(launched(launch_paged_attn_general(k.type, shared, st), "prefix attention"));
+    }
+    a.part0 = plan.prefix_splits;
+    a.splits = plan.splits;
+    TRY(launched(launch_paged_attn_general(k.type, a, st), "paged attention"));
+    if (plan.partial) TRY(launched(launch_paged_merge(k.type, a, plan.splits + plan.prefix_splits, st), "paged merge"));
+    return VOX_OK;
+}
+
+}  // namespace
+
+extern "C" int vox_paged_append_rope(const vox_paged_cache* c, const vox_paged_batch* b, const vox_rows* k_new,
+                                     const vox_rows* v_new, float theta, size_t n_heads, const vox_rows* q,
+                                     const vox_rows* q_out, void* stream) {
+    Checked k;
+    TRY(check_cache(c, &k));
+    TRY(check_batch(c, b));
+    if (theta != 0.f && !(theta >= 1.f && std::isfinite(theta)))
+        return report_errorf(VOX_ERR_INVALID_ARG, "rope_theta must be 0 or finite and >= 1");
+    if (q && (n_heads == 0 || n_heads > 65536)) return report_errorf(VOX_ERR_INVALID_ARG, "n_heads must be in 1..65536");
+    if (b->n_seqs == 0 || b->n_tokens == 0) return VOX_OK;
+    PagedAppendArgs a{};
+    fill_common(a, c, k, b);
+    a.k = c->keys;
+    a.v = c->values;
+    a.first_pos = b->first_pos;
+    TRY(check_rows(k_new, "k_new", b->n_tokens, c->n_kv_heads, c->head_dim, k.type, false, &a.kn_ts, &a.kn_hs));
+    TRY(check_rows(v_new, "v_new", b->n_tokens, c->n_kv_heads, c->head_dim, k.type, false, &a.vn_ts, &a.vn_hs));
+    a.k_new = k_new->ptr;
+    a.v_new = v_new->ptr;
+    if (q) {
+        TRY(check_rows(q, "q", b->n_tokens, n_heads, c->head_dim, k.type, false, &a.q_ts, &a.q_hs));
+        TRY(check_rows(q_out, "q_out", b->n_tokens, n_heads, c->head_dim, k.type, true, &a.qo_ts, &a.qo_hs));
+        a.q = q->ptr;
+        a.q_out = q_out->ptr;
+        a.n_heads = (int)n_heads;
+    }
+    a.rotate = theta != 0.f;
+    if (a.rotate) {
+        // theta^(-2c/D) / (2 pi) in units of 2^-64 turn, by repeated products in
+        // 64-bit-mantissa arithmetic
+        const long double ratio = powl((long double)theta, -2.0L / (long double)c->head_dim);
+        long double f = 0.15915494309189533576888376337251436L;
+        for (size_t i = 0; i < c->head_dim / 2; ++i, f *= ratio) a.turns[i] = (uint64_t)ldexpl(f, 64);
+    }
+    // 16-byte columns where every row starts on a 16-byte boundary
+    const bool wide = c->head_dim * type_size(k.type) % 16 == 0 &&
+                      aligned16(c->keys, k.type, {a.page_stride, a.head_stride, a.slot_stride}) &&
+                      aligned16(c->values, k.type, {}) && aligned16(a.k_new, k.type, {a.kn_ts, a.kn_hs}) &&
+                      aligned16(a.v_new, k.type, {a.vn_ts, a.vn_hs}) &&
+                      (!q || (aligned16(a.q, k.type, {a.q_ts, a.q_hs}) && aligned16(a.q_out, k.type, {a.qo_ts, a.qo_hs})));
+    DeviceGuard dev;
+    TRY(dev.enter(c->device));
+    return launched(launch_paged_append(k.type, a, wide, static_cast<cudaStream_t>(stream)), "paged append");
+}
+
+extern "C" int vox_paged_attention_workspace(const vox_paged_cache* c, const vox_paged_batch* b, size_t n_heads,
+                                             size_t window, size_t sinks, size_t* bytes) {
+    return attention_workspace(c, b, nullptr, n_heads, window, sinks, bytes);
+}
+
+extern "C" int vox_paged_attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_rows* q,
+                                   size_t n_heads, size_t window, size_t sinks, float scale, const vox_rows* out,
+                                   void* ws, size_t ws_bytes, void* stream) {
+    return attention(c, b, nullptr, q, n_heads, window, sinks, scale, out, ws, ws_bytes, stream);
+}
+
+extern "C" int vox_paged_prefix_attention_workspace(const vox_paged_cache* c, const vox_paged_batch* b,
+                                                    const vox_paged_prefix* p, size_t n_heads, size_t window,
+                                                    size_t sinks, size_t* bytes) {
+    if (!p) return report_errorf(VOX_ERR_INVALID_ARG, "null prefix");
+    return attention_workspace(c, b, p, n_heads, window, sinks, bytes);
+}
+
+extern "C" int vox_paged_prefix_attention(const vox_paged_cache* c, const vox_paged_batch* b,
+                                          const vox_paged_prefix* p, const vox_rows* q, size_t n_heads, size_t window,
+                                          size_t sinks, float scale, const vox_rows* out, void* ws, size_t ws_bytes,
+                                          void* stream) {
+    if (!p) return report_errorf(VOX_ERR_INVALID_ARG, "null prefix");
+    return attention(c, b, p, q, n_heads, window, sinks, scale, out, ws, ws_bytes, stream);
+}

@@ -1,0 +1,342 @@
+// vox_paged.cu -- paged key/value cache: the append with the position rotation
+// on the way, attention for any head dimension and alignment, and the joining
+// of partial results.
+#include "vox_paged.cuh"
+
+namespace vox {
+
+namespace {
+
+// ---- append -------------------------------------------------------------------
+//
+// Bound by bytes: every element is read once and written once.  One CTA of 256
+// threads per token: a thread owns one 16-byte column of the head dimension (its
+// pairs' sines and cosines are computed once) and walks over the heads of k, v
+// and q, four rows in flight.
+//
+// The angle a * theta^(-2c/D) matters modulo a turn only.  turns[c] is the turn
+// fraction per position as a 64-bit binary fraction, so the 64-bit product with
+// the position wraps exactly: the error is the position times 2^-64 of a turn,
+// whatever the position, without 64-bit floating point.  sincospif takes the
+// wrapped product as a signed 32-bit float (error 2^-25 of a half turn).
+
+template <class T, bool WIDE>
+struct alignas(WIDE ? 16 : sizeof(T)) AppendUnit {
+    static constexpr int N = WIDE ? 16 / (int)sizeof(T) : 2;
+    T v[N];
+};
+
+template <class T, bool WIDE>
+__device__ __forceinline__ AppendUnit<T, WIDE> append_load(const T* p) {
+    AppendUnit<T, WIDE> u;
+    if constexpr (WIDE) {
+        *reinterpret_cast<uint4*>(&u) = *reinterpret_cast<const uint4*>(p);
+    } else {
+        u.v[0] = p[0];
+        u.v[1] = p[1];
+    }
+    return u;
+}
+
+template <class T, bool WIDE>
+__device__ __forceinline__ void append_store(T* p, const AppendUnit<T, WIDE>& u) {
+    if constexpr (WIDE) {
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&u);
+    } else {
+        p[0] = u.v[0];
+        p[1] = u.v[1];
+    }
+}
+
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
+    constexpr int N = AppendUnit<T, WIDE>::N, P = N / 2, U = 4;
+    const int chunks = a.hd / N, heads_at_once = 256 / chunks;
+    const int c = threadIdx.x % chunks, h0 = threadIdx.x / chunks;
+    const int t = blockIdx.x;
+    const int rows = 2 * a.n_kv + (a.q ? a.n_heads : 0);  // k heads, v heads, q heads
+    const bool active = h0 < heads_at_once;
+
+    // where the token goes; the first rows are on their way meanwhile
+    AppendUnit<T, WIDE> u[U];
+    auto source = [&](int r) -> const T* {
+        if (r < a.n_kv) return static_cast<const T*>(a.k_new) + t * a.kn_ts + r * a.kn_hs;
+        if (r < 2 * a.n_kv) return static_cast<const T*>(a.v_new) + t * a.vn_ts + (r - a.n_kv) * a.vn_hs;
+        return static_cast<const T*>(a.q) + t * a.q_ts + (r - 2 * a.n_kv) * a.q_hs;
+    };
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int r = r0 + i * heads_at_once;
+            if (active && r < rows) u[i] = append_load<T, WIDE>(source(r) + c * N);
+        }
+    };
+    load(h0);
+
+    const int s = paged_seq_of_warp(a, t);
+    if (s < 0) return;
+    const PagedSeq q = paged_seq(a, s);
+    if (!q.ok) {
+        if (threadIdx.x == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        return;
+    }
+    if (t - q.q0 >= q.nq) return;  // behind the last sequence
+    const int p = q.len - q.nq + (t - q.q0);
+    int64_t slot = -1;
+    if (p >= 0) {
+        const int page = a.table[s * a.table_stride + (p >> a.page_shift)];
+        if ((unsigned)page < (unsigned)a.n_pages)
+            slot = page * a.page_stride + (p & ((1 << a.page_shift) - 1)) * a.slot_stride;
+        else if (threadIdx.x == 0)
+            paged_status(a, VOX_PAGED_BAD_PAGE);
+    }
+    float sn[P], cs[P];
+    if (a.rotate) {
+        const uint64_t pos = (uint64_t)((a.first_pos ? a.first_pos[s] : 0) + p);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (!active) break;
+            const int64_t turn = (int64_t)(pos * a.turns[c * P + i]);
+            sincospif((float)turn * 0x1p-63f, &sn[i], &cs[i]);
+        }
+    }
+    if (!active) return;
+    for (int r0 = h0; r0 < rows; r0 += U * heads_at_once) {
+        if (r0 != h0) load(r0);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int r = r0 + i * heads_at_once;
+            if (r >= rows) break;
+            const bool is_v = r >= a.n_kv && r < 2 * a.n_kv;
+            if (a.rotate && !is_v) {
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    const float x0 = to_f32(u[i].v[2 * j]), x1 = to_f32(u[i].v[2 * j + 1]);
+                    u[i].v[2 * j] = from_f32<T>(x0 * cs[j] - x1 * sn[j]);
+                    u[i].v[2 * j + 1] = from_f32<T>(x0 * sn[j] + x1 * cs[j]);
+                }
+            }
+            T* dst;
+            if (r >= 2 * a.n_kv)
+                dst = static_cast<T*>(a.q_out) + t * a.qo_ts + (r - 2 * a.n_kv) * a.qo_hs;
+            else if (slot < 0)
+                continue;
+            else if (is_v)
+                dst = static_cast<T*>(a.v) + slot + (r - a.n_kv) * a.head_stride;
+            else
+                dst = static_cast<T*>(a.k) + slot + r * a.head_stride;
+            append_store<T, WIDE>(dst + c * N, u[i]);
+        }
+    }
+}
+
+// ---- attention on the CUDA cores -------------------------------------------------
+//
+// For head dimensions and alignments that the tensor-core kernels do not take.
+// A CTA has 8 query rows (token x head of the kv head's group) and walks over
+// its share of the 32-key blocks that they see, with the running maximum and
+// sum of the softmax: scores by (row, key), values by dimension.  Everything is
+// f32 after the load.
+
+constexpr int kGenKeys = 32, kGenThreads = 128;
+
+size_t general_smem(int hd) { return sizeof(float) * ((size_t)kPagedGeneralRows * hd + kGenKeys * (hd + 1) + kGenKeys * hd); }
+
+template <class T>
+__global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int R = kPagedGeneralRows;
+    extern __shared__ float sm[];
+    const int hd = a.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    float* q_s = sm;                    // [R][hd]
+    float* k_s = q_s + R * hd;          // [32][hd + 1]
+    float* v_s = k_s + kGenKeys * (hd + 1);  // [32][hd]
+    __shared__ PagedTileRows<R> rows;
+    __shared__ float p_s[R][kGenKeys], alpha_s[R], l_s[R], m_s[R];
+    __shared__ int64_t off_s[kGenKeys];
+
+    const int z = blockIdx.x % a.splits;
+    const int h = (blockIdx.x / a.splits) % a.n_kv;
+    const int tile = blockIdx.x / a.splits / a.n_kv;
+    PagedKeys ks;
+    if (!paged_tile_rows(a, tile, rows, &ks)) return;
+    for (int i = tid; i < R * hd; i += kGenThreads) {
+        const int r = i / hd, d = i % hd;
+        float x = 0.f;
+        if (rows.tok[r] >= 0)
+            x = to_f32(static_cast<const T*>(a.q)[rows.tok[r] * a.q_ts + (h * a.group + rows.g[r]) * a.q_hs + d]);
+        q_s[i] = x;
+    }
+    const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 5);
+    const int b0 = (int)((int64_t)kb.total * z / a.splits), b1 = (int)((int64_t)kb.total * (z + 1) / a.splits);
+
+    float acc[R][2] = {};
+    float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};  // rows warp and warp + 4
+    for (int b = b0; b < b1; ++b) {
+        const int j0 = kb.block(b) * kGenKeys;
+        __syncthreads();  // the previous block's values are used up
+        if (tid < kGenKeys) off_s[tid] = kb.seen(j0 + tid) ? paged_row(a, ks, j0 + tid, h) : -1;
+        __syncthreads();
+        for (int i = tid; i < kGenKeys * hd; i += kGenThreads) {
+            const int j = i / hd, d = i % hd;
+            const int64_t o = off_s[j];
+            k_s[j * (hd + 1) + d] = o >= 0 ? to_f32(static_cast<const T*>(a.k)[o + d]) : 0.f;
+            v_s[i] = o >= 0 ? to_f32(static_cast<const T*>(a.v)[o + d]) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = warp + 4 * i;
+            float s = 0.f;
+            for (int d = 0; d < hd; ++d) s = fmaf(q_s[r * hd + d], k_s[lane * (hd + 1) + d], s);
+            const bool seen = rows.tok[r] >= 0 && paged_sees(rows.p[r], j0 + lane, ks.len, a.window, ks.sinks);
+            s = seen ? s * a.scale_log2 : kNegInf;
+            float top = s;
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+            const float m_new = fmaxf(m[i], top), base = m_new == kNegInf ? 0.f : m_new;
+            const float pr = seen ? exp2f(s - base) : 0.f;
+            float sum = pr;
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            const float alpha = exp2f(m[i] - base);
+            l[i] = l[i] * alpha + sum;
+            m[i] = m_new;
+            p_s[r][lane] = pr;
+            if (lane == 0) alpha_s[r] = alpha;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = tid + e * kGenThreads;
+            if (d < hd) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r][e] *= alpha_s[r];
+                for (int j = 0; j < kGenKeys; ++j) {
+                    const float x = v_s[j * hd + d];
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {  // a weight of 0 takes nothing from a value, finite or not
+                        const float pr = p_s[r][j];
+                        acc[r][e] = pr != 0.f ? fmaf(pr, x, acc[r][e]) : acc[r][e];
+                    }
+                }
+            }
+        }
+    }
+    if (lane == 0) {
+        l_s[warp] = l[0], l_s[warp + 4] = l[1];
+        m_s[warp] = m[0], m_s[warp + 4] = m[1];
+    }
+    __syncthreads();
+    for (int r = 0; r < R; ++r) {
+        const int tok = rows.tok[r];
+        if (tok < 0) continue;
+        const int head = h * a.group + rows.g[r];
+        const float ls = l_s[r];
+        const int64_t at = ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head;
+        if (a.part_o && tid == 0) a.part_ml[at] = make_float2(m_s[r], ls);
+        for (int e = 0; e < 2; ++e) {
+            const int d = tid + e * kGenThreads;
+            if (d >= hd) break;
+            if (a.part_o)
+                a.part_o[at * hd + d] = acc[r][e];
+            else
+                static_cast<T*>(a.out)[tok * a.o_ts + head * a.o_hs + d] = from_f32<T>(ls == 0.f ? 0.f : acc[r][e] / ls);
+        }
+    }
+}
+
+// ---- joining partial results -----------------------------------------------------
+//
+// out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in the order of the
+// parts.  One warp per (token, head); a part whose sum is 0 is not read.
+
+template <class T>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a, int n_parts) {
+    const int64_t n_rows = (int64_t)a.n_tokens * a.n_heads;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int tok = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
+    bool mine = row < n_rows && !(a.pfx_len && paged_prefix_len(a) < 0);
+    if (mine) {
+        const int s = paged_seq_of_warp(a, tok);
+        const PagedSeq q = s >= 0 ? paged_seq(a, s) : PagedSeq{};
+        mine = s >= 0 && tok - q.q0 < q.nq;
+    }
+    pdl_wait_prior_grids();
+    if (!mine) return;
+    float top = kNegInf;
+    for (int i = lane; i < n_parts; i += 32) {
+        const float2 ml = a.part_ml[i * n_rows + row];
+        top = fmaxf(top, ml.x);
+    }
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const float base = top == kNegInf ? 0.f : top;
+    float total = 0.f, acc[kPagedMaxHeadDim / 32] = {};
+    for (int i = 0; i < n_parts; ++i) {
+        const float2 ml = a.part_ml[i * n_rows + row];
+        if (ml.y == 0.f) continue;
+        const float w = exp2f(ml.x - base);
+        total = fmaf(w, ml.y, total);
+        const float* o = a.part_o + (i * n_rows + row) * a.hd;
+#pragma unroll
+        for (int e = 0; e < kPagedMaxHeadDim / 32; ++e)
+            if (lane + 32 * e < a.hd) acc[e] = fmaf(w, o[lane + 32 * e], acc[e]);
+    }
+    T* out = static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs;
+#pragma unroll
+    for (int e = 0; e < kPagedMaxHeadDim / 32; ++e)
+        if (lane + 32 * e < a.hd) out[lane + 32 * e] = from_f32<T>(total == 0.f ? 0.f : acc[e] / total);
+}
+
+template <class F>
+cudaError_t by_type(PagedType t, F f) {
+    switch (t) {
+        case PagedType::F32: return f(float{});
+        case PagedType::F16: return f(__half{});
+        case PagedType::BF16: return f(__nv_bfloat16{});
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_paged_append(PagedType t, const PagedAppendArgs& a, bool wide, cudaStream_t st) {
+    return by_type(t, [&](auto x) {
+        using T = decltype(x);
+        if (wide)
+            paged_append_kernel<T, true><<<a.n_tokens, 256, 0, st>>>(a);
+        else
+            paged_append_kernel<T, false><<<a.n_tokens, 256, 0, st>>>(a);
+        return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_paged_attn_general(PagedType t, const PagedAttnArgs& a, cudaStream_t st) {
+    const int64_t grid = paged_tiles_bound(a, kPagedGeneralRows) * a.n_kv * a.splits;
+    if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    const size_t smem = general_smem(a.hd);
+    return by_type(t, [&](auto x) {
+        auto* k = paged_attn_general_kernel<decltype(x)>;
+        if (smem > 48 * 1024) {
+            cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return e;
+        }
+        k<<<(unsigned)grid, kGenThreads, smem, st>>>(a);
+        return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_paged_merge(PagedType t, const PagedAttnArgs& a, int n_parts, cudaStream_t st) {
+    const int64_t grid = ((int64_t)a.n_tokens * a.n_heads + 3) / 4;
+    if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return by_type(t, [&](auto x) { return cudaLaunchKernelEx(&cfg, paged_merge_kernel<decltype(x)>, a, n_parts); });
+}
+
+}  // namespace vox

@@ -1,0 +1,256 @@
+// vox_paged.cuh -- device helpers of the paged-cache kernels: checked batch
+// metadata, the list of key blocks a tile of query rows sees, masks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/vox_decoder.h"
+#include "vox_device.cuh"
+#include "vox_paged.h"
+
+namespace vox {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// 2^x on the special-function unit (relative error about 2^-22); 0 for -inf.
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct PagedSeq {
+    int q0, nq, len;  // first token, tokens of the call, cached tokens
+    bool ok;          // false: bad lengths, the sequence is skipped (nq 0)
+};
+
+// A sequence's lengths, checked against the host's bounds (A: either argument struct).
+template <class A>
+__device__ __forceinline__ PagedSeq paged_seq(const A& a, int s) {
+    const int q0 = a.q_start[s], q1 = a.q_start[s + 1], len = a.kv_len[s];
+    PagedSeq r;
+    r.ok = q0 >= 0 && q1 >= q0 && q1 <= a.n_tokens && q1 - q0 <= a.max_q && len >= 0 && len <= a.max_kv &&
+           (len >> a.page_shift) + ((len & ((1 << a.page_shift) - 1)) != 0) <= a.table_width;
+    r.q0 = q0;
+    r.nq = r.ok ? q1 - q0 : 0;
+    r.len = len;
+    return r;
+}
+
+template <class A>
+__device__ __forceinline__ void paged_status(const A& a, uint32_t bit) {
+    if (a.status) atomicOr(a.status, bit);
+}
+
+// The sequence whose tokens hold token t: the last s with q_start[s] <= t
+// (-1: none).  The caller still checks that t lies in it.
+template <class A>
+__device__ __forceinline__ int paged_seq_of(const A& a, int t) {
+    int lo = 0, hi = a.n_seqs;  // first s in [0, n_seqs) with q_start[s] > t
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.q_start[mid] > t) hi = mid; else lo = mid + 1;
+    }
+    return lo - 1;
+}
+
+// The prefix's length, or -1 where it is out of its bounds.
+__device__ __forceinline__ int paged_prefix_len(const PagedAttnArgs& a) {
+    const int n = *a.pfx_len;
+    const int pages = (n >> a.page_shift) + ((n & ((1 << a.page_shift) - 1)) != 0);
+    return n < 0 || n > a.pfx_max || pages > a.pfx_n_pages ? -1 : n;
+}
+
+// Tile `t` of the tiles of `rows` query rows (a sequence's row is token * group
+// + head) that cover every sequence in turn; one warp calls it.  Returns the
+// sequence (-1: none) and the tile's place in it.
+__device__ __forceinline__ int paged_find_tile(const PagedAttnArgs& a, int t, int rows, int* place) {
+    const int lane = threadIdx.x & 31;
+    if ((int64_t)a.max_q * a.group <= rows) {  // at most one tile a sequence
+        *place = 0;
+        return t < a.n_seqs ? t : -1;
+    }
+    int before = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < a.n_seqs) {
+            const PagedSeq q = paged_seq(a, s);
+            if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);  // no tile stands for it
+            n = (int)(((int64_t)q.nq * a.group + rows - 1) / rows);
+        }
+        int sum = n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += up;
+        }
+        const unsigned hit = __ballot_sync(~0u, before + sum > t);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            *place = t - before - __shfl_sync(~0u, sum - n, src);
+            return s0 + src;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+    }
+    *place = 0;
+    return -1;
+}
+
+// Upper bound on those tiles, from the host's bounds alone.
+inline int64_t paged_tiles_bound(const PagedAttnArgs& a, int rows) {
+    if (a.in_prefix) return ((int64_t)a.n_tokens * a.group + rows - 1) / rows;
+    if ((int64_t)a.max_q * a.group <= rows) return a.n_seqs;
+    return (int64_t)a.n_tokens * a.group / rows + a.n_seqs;
+}
+
+// The blocks of 2^shift keys that some row with an index in [pmin, pmax] sees,
+// among keys 0..len-1: the sinks' blocks, then the window's.
+struct KeyBlocks {
+    int sink_blocks, first, total;  // total blocks; the window's begin with `first`
+    int end, lo, sinks;             // keys [0, min(sinks, end)) and [lo, end) are seen
+    __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : first + i - sink_blocks; }
+    __device__ __forceinline__ bool seen(int j) const { return j < end && (j >= lo || j < sinks); }
+};
+__device__ __forceinline__ KeyBlocks paged_key_blocks(int pmin, int pmax, int len, int window, int sinks, int shift) {
+    KeyBlocks b;
+    b.end = min(pmax, len - 1) + 1;
+    if (b.end < 0) b.end = 0;
+    b.lo = window ? max(0, pmin - window + 1) : 0;
+    b.sinks = b.lo ? sinks : 0;
+    const int mask = (1 << shift) - 1;
+    const int nb = (b.end >> shift) + ((b.end & mask) != 0);
+    const int se = min(b.sinks, b.end);
+    b.sink_blocks = (se >> shift) + ((se & mask) != 0);
+    b.first = max(b.lo >> shift, b.sink_blocks);
+    b.total = b.sink_blocks + max(0, nb - b.first);
+    return b;
+}
+
+// Whether the token with index p sees key j (of keys 0..len-1).
+__device__ __forceinline__ bool paged_sees(int p, int j, int len, int window, int sinks) {
+    return j <= p && j < len && (window == 0 || j < sinks || j > p - window);
+}
+
+// What a tile of rows attends to: its table row, length and sink count.
+struct PagedKeys {
+    const int32_t* table;
+    int len, sinks;
+};
+
+// Offset of key j's row of kv head h, or -1 where its page id is bad.
+__device__ __forceinline__ int64_t paged_row(const PagedAttnArgs& a, const PagedKeys& ks, int j, int h) {
+    const int page = ks.table[j >> a.page_shift];
+    if ((unsigned)page >= (unsigned)a.n_pages) {
+        paged_status(a, VOX_PAGED_BAD_PAGE);
+        return -1;
+    }
+    return page * a.page_stride + h * a.head_stride + (j & ((1 << a.page_shift) - 1)) * a.slot_stride;
+}
+
+// A tile's query rows: token (-1: no such row), index in the keys' numbering,
+// head within the kv head's group.
+template <int ROWS>
+struct PagedTileRows {
+    int tok[ROWS], p[ROWS], g[ROWS];
+    int seq, place, pmin, pmax;
+};
+
+// Fills the rows of tile `tile` (in shared memory) and what they attend to.
+// All threads of the block call it (at least ROWS and at least a warp);
+// false, for the whole block alike: the tile has no rows.
+template <int ROWS>
+__device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile, PagedTileRows<ROWS>& rows,
+                                                PagedKeys* ks) {
+    const int tid = threadIdx.x;
+    const int plen = a.pfx_len ? paged_prefix_len(a) : 0;
+    if (plen < 0) {
+        if (tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        return false;
+    }
+    if (tid == 0) rows.pmin = 0x7FFFFFFF, rows.pmax = -0x7FFFFFFF;
+    int tok = -1, p = -1;
+    int64_t row;
+    if (!a.in_prefix) {
+        if (tid < 32) {
+            int place;
+            const int s = paged_find_tile(a, tile, ROWS, &place);
+            if (tid == 0) rows.seq = s, rows.place = place;
+        }
+        __syncthreads();
+        const int s = rows.seq;
+        if (s < 0) return false;
+        const PagedSeq q = paged_seq(a, s);
+        if (!q.ok && tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        if (q.nq == 0) return false;
+        row = (int64_t)rows.place * ROWS + tid;
+        if (tid < ROWS && row < (int64_t)q.nq * a.group) {
+            const int i = (int)(row / a.group);
+            tok = q.q0 + i;
+            p = q.len - q.nq + i;
+        }
+        ks->table = a.table + s * a.table_stride;
+        ks->len = q.len;
+        ks->sinks = max(0, a.sinks - plen);
+    } else {
+        __syncthreads();
+        row = (int64_t)tile * ROWS + tid;
+        if (tid < ROWS && row < (int64_t)a.n_tokens * a.group) {
+            const int t = (int)(row / a.group);
+            const int s = paged_seq_of(a, t);
+            if (s >= 0) {
+                const PagedSeq q = paged_seq(a, s);
+                if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);
+                if (t - q.q0 < q.nq) tok = t, p = plen + q.len - q.nq + (t - q.q0);
+            }
+        }
+        ks->table = a.pfx_pages;
+        ks->len = plen;
+        ks->sinks = a.sinks;
+    }
+    if (tid < ROWS) {
+        rows.tok[tid] = tok;
+        rows.p[tid] = p;
+        rows.g[tid] = (int)(row % a.group);
+        if (tok >= 0) {
+            atomicMin(&rows.pmin, p);
+            atomicMax(&rows.pmax, p);
+        }
+    }
+    __syncthreads();
+    return rows.pmin <= rows.pmax;
+}
+
+// paged_seq_of for a whole warp: 32 probes at a time.
+template <class A>
+__device__ __forceinline__ int paged_seq_of_warp(const A& a, int t) {
+    int lo = 0, n = a.n_seqs;  // the first s with q_start[s] > t lies in [lo, lo + n]
+    const int lane = threadIdx.x & 31;
+    while (n > 0) {
+        const int step = (n + 31) >> 5;
+        const int i = lane * step + step - 1;  // last of this lane's share
+        const bool past = i >= n || a.q_start[lo + i] > t;
+        const unsigned hit = __ballot_sync(~0u, past);
+        const int c = hit ? __ffs(hit) - 1 : 32;
+        if (c * step >= n) {
+            lo += n;
+            break;
+        }
+        lo += c * step;
+        // a probe inside the range found its share's last entry past t already
+        n = c * step + step <= n ? step - 1 : n - c * step;
+    }
+    return lo - 1;
+}
+
+}  // namespace vox

@@ -1,0 +1,79 @@
+// vox_paged.h -- what the paged-cache host file (vox_paged.cpp) and its kernels
+// (vox_paged*.cu) share: launch arguments and launchers.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace vox {
+
+enum class PagedType : int { F32, F16, BF16 };
+
+constexpr int kPagedMaxHeadDim = 256;
+
+// Arguments of every paged attention kernel.  Counts and token indices are
+// 32 bits (the host checks them); every offset into a tensor is 64 bits.
+struct PagedAttnArgs {
+    // pool
+    const void* k;
+    const void* v;
+    int64_t page_stride, head_stride, slot_stride;
+    int n_pages, page_shift, n_kv, hd;
+    // batch
+    int n_seqs, n_tokens, max_q, max_kv, table_width;
+    int64_t table_stride;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    const int32_t* table;
+    uint32_t* status;
+    // shared prefix (pfx_len null: none).  in_prefix 1: the keys are the
+    // prefix's and the rows all tokens of the batch; 0: each sequence's own.
+    const int32_t* pfx_pages;
+    const int32_t* pfx_len;
+    int pfx_n_pages, pfx_max, in_prefix;
+    // queries and outputs
+    const void* q;
+    int64_t q_ts, q_hs;
+    void* out;
+    int64_t o_ts, o_hs;
+    int n_heads, group;
+    float scale_log2;   // score scale * log2(e): softmax runs on powers of two
+    int window, sinks;  // window 0 = none
+    // partial results (part_o null: the kernel writes `out`).  This launch
+    // writes the parts part0 .. part0 + splits - 1 of [part][token][head].
+    float* part_o;
+    float2* part_ml;  // (maximum score in log2 units, sum)
+    int part0, splits;
+};
+
+struct PagedAppendArgs {
+    void* k;
+    void* v;
+    int64_t page_stride, head_stride, slot_stride;
+    int n_pages, page_shift, n_kv, hd;
+    int n_seqs, n_tokens, max_q, max_kv, table_width;
+    int64_t table_stride;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    const int32_t* table;
+    const int64_t* first_pos;
+    uint32_t* status;
+    const void *k_new, *v_new, *q;
+    void* q_out;
+    int64_t kn_ts, kn_hs, vn_ts, vn_hs, q_ts, q_hs, qo_ts, qo_hs;
+    int n_heads, rotate;
+    // theta^(-2c/hd) / (2 pi) as a 64-bit binary fraction of a turn
+    uint64_t turns[kPagedMaxHeadDim / 2];
+};
+
+cudaError_t launch_paged_append(PagedType t, const PagedAppendArgs& a, bool wide, cudaStream_t st);
+
+// CUDA-core attention: any head_dim and alignment (vox_paged.cu).
+cudaError_t launch_paged_attn_general(PagedType t, const PagedAttnArgs& a, cudaStream_t st);
+constexpr int kPagedGeneralRows = 8;  // query rows (token x head of a group) of a CTA
+
+// Joins n_parts partial results into `out` (vox_paged.cu).
+cudaError_t launch_paged_merge(PagedType t, const PagedAttnArgs& a, int n_parts, cudaStream_t st);
+
+}  // namespace vox
