@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/vox_decoder.h"
 #include "vox_host.h"
@@ -170,30 +171,84 @@ void fill_common(A& a, const vox_paged_cache* c, const Checked& k, const vox_pag
     a.status = b->status;
 }
 
-// What a call launches, from the host's bounds.
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// How one set of keys (the sequences' own, or the prefix) is attended to.  It
+// follows from the host's bounds and the head dimension alone; a call whose
+// tensors are not on 16-byte boundaries takes the CUDA-core kernel with the
+// same splits.
+struct KeysPlan {
+    bool rows = false;  // the tensor-core kernel for few rows (else the CUDA cores)
+    int nt = 1, cluster = 1, splits = 1;
+};
+
+// `rows`: query rows of a tile set (a sequence's, or all); `tiles(n)`: tiles of
+// n rows; `keys`: keys that a row can see.
+template <class F>
+KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t keys, F tiles) {
+    KeysPlan p;
+    p.rows = c->head_dim == 64 || c->head_dim == 128;
+    p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    const int64_t units = std::max<int64_t>(1, tiles(p.rows ? 8 * p.nt : kPagedGeneralRows) * (int64_t)c->n_kv_heads);
+    // CTAs that run at once.  Fewer tiles than that are split into one wave of
+    // equal shares; more, where the bytes bound the call (one decode step's rows),
+    // into about four waves, which evens out ragged lengths: 96 sequences of up
+    // to 8192 visible keys 411 us against 434 with half as many CTAs.
+    const int64_t slots = 148 * (t != PagedType::F32 || p.nt == 1 ? 2 : 1);
+    const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (4 * slots + units - 1) / units : 1;
+    // at least 64 keys to a CTA of a cluster (one stream of 1536 tokens: 15 us
+    // through clusters alone, 20 us with a merge behind them), 512 where the
+    // parts go through the merge
+    int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / 64));
+    if (p.rows)
+        while (p.cluster < 16 && 2 * p.cluster <= parts) p.cluster *= 2;
+    parts = std::min<int64_t>(parts / p.cluster, keys / 512 / p.cluster);
+    p.splits = (int)std::min<int64_t>(std::max<int64_t>(1, parts), 64);
+    return p;
+}
+
+// What a call launches.
 struct AttnPlan {
-    int splits = 1;         // parts of the sequences' own keys
-    int prefix_splits = 0;  // parts of the shared prefix's
-    bool partial = false;   // through the workspace
+    KeysPlan own, prefix;
+    int parts = 1;         // partial results of a row
+    bool partial = false;  // through the workspace
     size_t ml_bytes = 0, bytes = 0;
 };
 
-size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
-
-AttnPlan plan_attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_paged_prefix* p, size_t n_heads,
-                        size_t window, size_t sinks) {
+AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_batch* b, const vox_paged_prefix* p,
+                        size_t n_heads, size_t window, size_t sinks) {
     AttnPlan plan;
-    (void)window;
-    (void)sinks;
-    plan.splits = 1;
-    plan.prefix_splits = p ? 1 : 0;
-    plan.partial = plan.splits + plan.prefix_splits > 1;
+    const int64_t group = (int64_t)(n_heads / c->n_kv_heads);
+    auto visible = [&](size_t len) {
+        return (int64_t)(window ? std::min(len, window + b->max_q_len + std::min(sinks, len)) : len);
+    };
+    PagedAttnArgs a{};
+    a.n_tokens = (int)b->n_tokens;
+    a.n_seqs = (int)b->n_seqs;
+    a.max_q = (int)b->max_q_len;
+    a.group = (int)group;
+    plan.own = plan_keys(c, t, (int64_t)b->max_q_len * group, visible(b->max_kv_len),
+                         [&](int n) { return paged_tiles_bound(a, n); });
+    plan.parts = plan.own.splits;
+    if (p) {
+        a.in_prefix = 1;
+        plan.prefix = plan_keys(c, t, (int64_t)b->n_tokens * group, visible(p->max_len),
+                                [&](int n) { return paged_tiles_bound(a, n); });
+        plan.parts += plan.prefix.splits;
+    }
+    plan.partial = plan.parts > 1;
     if (plan.partial) {
-        const size_t rows = (size_t)(plan.splits + plan.prefix_splits) * b->n_tokens * n_heads;
+        const size_t rows = (size_t)plan.parts * b->n_tokens * n_heads;
         plan.ml_bytes = round256(rows * sizeof(float2));
         plan.bytes = plan.ml_bytes + rows * c->head_dim * sizeof(float);
     }
     return plan;
+}
+
+cudaError_t launch_keys(PagedType t, PagedAttnArgs& a, const KeysPlan& p, bool aligned, cudaStream_t st) {
+    a.splits = p.splits;
+    if (p.rows && aligned) return launch_paged_attn_rows(t, a, p.nt, p.cluster, st);
+    return launch_paged_attn_general(t, a, st);
 }
 
 int check_attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_paged_prefix* p, size_t n_heads,
@@ -217,7 +272,7 @@ int attention_workspace(const vox_paged_cache* c, const vox_paged_batch* b, cons
     if (!bytes) return report_errorf(VOX_ERR_INVALID_ARG, "null bytes");
     Checked k;
     TRY(check_attention(c, b, p, n_heads, &k));
-    *bytes = b->n_seqs && b->n_tokens ? plan_attention(c, b, p, n_heads, window, sinks).bytes : 0;
+    *bytes = b->n_seqs && b->n_tokens ? plan_attention(c, k.type, b, p, n_heads, window, sinks).bytes : 0;
     return VOX_OK;
 }
 
@@ -247,7 +302,7 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
         a.pfx_n_pages = (int)p->n_pages;
         a.pfx_max = (int)p->max_len;
     }
-    const AttnPlan plan = plan_attention(c, b, p, n_heads, window, sinks);
+    const AttnPlan plan = plan_attention(c, k.type, b, p, n_heads, window, sinks);
     if (plan.partial) {
         if (!ws || ws_bytes < plan.bytes || ((uintptr_t)ws & 255))
             return report_errorf(VOX_ERR_INVALID_ARG, "workspace must be %zu bytes, 256-byte aligned", plan.bytes);
@@ -257,16 +312,17 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
     DeviceGuard dev;
     TRY(dev.enter(c->device));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool aligned = aligned16(a.k, k.type, {a.page_stride, a.head_stride, a.slot_stride}) &&
+                         aligned16(a.v, k.type, {}) && aligned16(a.q, k.type, {a.q_ts, a.q_hs}) &&
+                         aligned16(a.out, k.type, {a.o_ts, a.o_hs});
     if (p) {
         PagedAttnArgs shared = a;
         shared.in_prefix = 1;
-        shared.splits = plan.prefix_splits;
-        TRY(launched(launch_paged_attn_general(k.type, shared, st), "prefix attention"));
+        TRY(launched(launch_keys(k.type, shared, plan.prefix, aligned, st), "prefix attention"));
+        a.part0 = plan.prefix.splits;
     }
-    a.part0 = plan.prefix_splits;
-    a.splits = plan.splits;
-    TRY(launched(launch_paged_attn_general(k.type, a, st), "paged attention"));
-    if (plan.partial) TRY(launched(launch_paged_merge(k.type, a, plan.splits + plan.prefix_splits, st), "paged merge"));
+    TRY(launched(launch_keys(k.type, a, plan.own, aligned, st), "paged attention"));
+    if (plan.partial) TRY(launched(launch_paged_merge(k.type, a, plan.parts, st), "paged merge"));
     return VOX_OK;
 }
 

@@ -107,13 +107,6 @@ __device__ __forceinline__ int paged_find_tile(const PagedAttnArgs& a, int t, in
     return -1;
 }
 
-// Upper bound on those tiles, from the host's bounds alone.
-inline int64_t paged_tiles_bound(const PagedAttnArgs& a, int rows) {
-    if (a.in_prefix) return ((int64_t)a.n_tokens * a.group + rows - 1) / rows;
-    if ((int64_t)a.max_q * a.group <= rows) return a.n_seqs;
-    return (int64_t)a.n_tokens * a.group / rows + a.n_seqs;
-}
-
 // The blocks of 2^shift keys that some row with an index in [pmin, pmax] sees,
 // among keys 0..len-1: the sinks' blocks, then the window's.
 struct KeyBlocks {
@@ -156,6 +149,37 @@ __device__ __forceinline__ int64_t paged_row(const PagedAttnArgs& a, const Paged
         return -1;
     }
     return page * a.page_stride + h * a.head_stride + (j & ((1 << a.page_shift) - 1)) * a.slot_stride;
+}
+
+// One row again, key by key: acc[e] = sum of 2^(score - m) v[lane + 32 e] over
+// the keys that the row sees among blocks b0..b1-1 of `keys` keys.  For rows
+// whose result is not finite; one warp calls it.
+template <class T, int E>
+__device__ __noinline__ void paged_redo_row(const PagedAttnArgs& a, PagedKeys ks, KeyBlocks kb, int keys, int b0, int b1,
+                                            int h, int tok, int head, int p, float m, float (&acc)[E]) {
+    const int lane = threadIdx.x & 31;
+    float q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        q[e] = to_f32(static_cast<const T*>(a.q)[tok * a.q_ts + head * a.q_hs + lane + 32 * e]);
+        acc[e] = 0.f;
+    }
+    const float base = m == kNegInf ? 0.f : m;
+    for (int b = b0; b < b1; ++b)
+        for (int i = 0; i < keys; ++i) {
+            const int j = kb.block(b) * keys + i;
+            if (!paged_sees(p, j, ks.len, a.window, ks.sinks)) continue;
+            const int64_t off = paged_row(a, ks, j, h);
+            if (off < 0) continue;  // zeros: adds nothing
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f32(static_cast<const T*>(a.k)[off + lane + 32 * e]), s);
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+            const float w = fast_exp2(s * a.scale_log2 - base);
+            if (w == 0.f) continue;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, to_f32(static_cast<const T*>(a.v)[off + lane + 32 * e]), acc[e]);
+        }
 }
 
 // A tile's query rows: token (-1: no such row), index in the keys' numbering,

@@ -47,6 +47,13 @@ struct PagedAttnArgs {
     int part0, splits;
 };
 
+// Upper bound on the tiles of `rows` query rows, from the host's bounds alone.
+inline int64_t paged_tiles_bound(const PagedAttnArgs& a, int rows) {
+    if (a.in_prefix) return ((int64_t)a.n_tokens * a.group + rows - 1) / rows;
+    if ((int64_t)a.max_q * a.group <= rows) return a.n_seqs;
+    return (int64_t)a.n_tokens * a.group / rows + a.n_seqs;
+}
+
 struct PagedAppendArgs {
     void* k;
     void* v;
@@ -72,6 +79,11 @@ cudaError_t launch_paged_append(PagedType t, const PagedAppendArgs& a, bool wide
 // CUDA-core attention: any head_dim and alignment (vox_paged.cu).
 cudaError_t launch_paged_attn_general(PagedType t, const PagedAttnArgs& a, cudaStream_t st);
 constexpr int kPagedGeneralRows = 8;  // query rows (token x head of a group) of a CTA
+
+// Tensor-core attention for few rows per key (vox_paged_rows.cu): head_dim 64 or
+// 128, every row on a 16-byte boundary; nt (1, 2, 4) x 8 query rows per tile,
+// `cluster` (1..16) CTAs per tile and part.
+cudaError_t launch_paged_attn_rows(PagedType t, const PagedAttnArgs& a, int nt, int cluster, cudaStream_t st);
 
 // Joins n_parts partial results into `out` (vox_paged.cu).
 cudaError_t launch_paged_merge(PagedType t, const PagedAttnArgs& a, int n_parts, cudaStream_t st);
