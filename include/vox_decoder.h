@@ -612,6 +612,7 @@ typedef struct vox_paged_batch {
 } vox_paged_batch;
 #define VOX_PAGED_BAD_LENGTH 1u
 #define VOX_PAGED_BAD_PAGE 2u
+#define VOX_PAGED_TIMEOUT 4u /* a bounded wait inside a kernel expired: the outputs are incomplete */
 /* [n_tokens, heads, head_dim] with a unit last stride; both strides 0 = packed. */
 typedef struct vox_rows {
     void* ptr;

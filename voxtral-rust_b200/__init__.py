@@ -150,7 +150,7 @@ class Rows(C.Structure):
     _fields_ = [("ptr", VP), ("token_stride", SZ), ("head_stride", SZ)]
 
 
-PAGED_BAD_LENGTH, PAGED_BAD_PAGE = 1, 2
+PAGED_BAD_LENGTH, PAGED_BAD_PAGE, PAGED_TIMEOUT = 1, 2, 4
 
 _lib = None
 

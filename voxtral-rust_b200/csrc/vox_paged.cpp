@@ -178,7 +178,7 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 // tensors are not on 16-byte boundaries takes the CUDA-core kernel with the
 // same splits.
 struct KeysPlan {
-    bool rows = false;  // the tensor-core kernel for few rows (else the CUDA cores)
+    enum Kernel { GENERAL, ROWS, TILES } kernel = GENERAL;
     int nt = 1, cluster = 1, splits = 1;
 };
 
@@ -187,9 +187,18 @@ struct KeysPlan {
 template <class F>
 KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t keys, F tiles) {
     KeysPlan p;
-    p.rows = c->head_dim == 64 || c->head_dim == 128;
+    const bool fits = c->head_dim == 64 || c->head_dim == 128;
+    // tcgen05 tiles have 128 rows: from 32 rows on they win although part of
+    // them is empty (the rows' kernel reads K and V again for every 32 rows)
+    if (fits && rows > 32 && t != PagedType::F32 && c->page_size >= 8) {
+        p.kernel = KeysPlan::TILES;
+        const int64_t units = std::max<int64_t>(1, tiles(kPagedTileRows) * (int64_t)c->n_kv_heads);
+        p.splits = (int)std::min<int64_t>(std::max<int64_t>(1, std::min<int64_t>(148 / units, keys / 256)), 64);
+        return p;
+    }
+    if (fits) p.kernel = KeysPlan::ROWS;
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    const int64_t units = std::max<int64_t>(1, tiles(p.rows ? 8 * p.nt : kPagedGeneralRows) * (int64_t)c->n_kv_heads);
+    const int64_t units = std::max<int64_t>(1, tiles(fits ? 8 * p.nt : kPagedGeneralRows) * (int64_t)c->n_kv_heads);
     // CTAs that run at once.  Fewer tiles than that are split into one wave of
     // equal shares; more, where the bytes bound the call (one decode step's rows),
     // into about four waves, which evens out ragged lengths: 96 sequences of up
@@ -200,7 +209,7 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     // through clusters alone, 20 us with a merge behind them), 512 where the
     // parts go through the merge
     int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / 64));
-    if (p.rows)
+    if (fits)
         while (p.cluster < 16 && 2 * p.cluster <= parts) p.cluster *= 2;
     parts = std::min<int64_t>(parts / p.cluster, keys / 512 / p.cluster);
     p.splits = (int)std::min<int64_t>(std::max<int64_t>(1, parts), 64);
@@ -247,7 +256,9 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
 
 cudaError_t launch_keys(PagedType t, PagedAttnArgs& a, const KeysPlan& p, bool aligned, cudaStream_t st) {
     a.splits = p.splits;
-    if (p.rows && aligned) return launch_paged_attn_rows(t, a, p.nt, p.cluster, st);
+    if (p.kernel == KeysPlan::TILES && aligned && std::max({a.page_stride, a.head_stride, a.slot_stride}) < (int64_t(1) << 39))
+        return launch_paged_attn_tiles(t, a, st);
+    if (p.kernel == KeysPlan::ROWS && aligned) return launch_paged_attn_rows(t, a, p.nt, p.cluster, st);
     return launch_paged_attn_general(t, a, st);
 }
 

@@ -85,6 +85,11 @@ constexpr int kPagedGeneralRows = 8;  // query rows (token x head of a group) of
 // `cluster` (1..16) CTAs per tile and part.
 cudaError_t launch_paged_attn_rows(PagedType t, const PagedAttnArgs& a, int nt, int cluster, cudaStream_t st);
 
+// tcgen05 attention for many rows per key (vox_paged_tiles.cu): f16 and bf16,
+// head_dim 64 or 128, pages of at least 8 slots, every row on a 16-byte boundary.
+cudaError_t launch_paged_attn_tiles(PagedType t, const PagedAttnArgs& a, cudaStream_t st);
+constexpr int kPagedTileRows = 256;  // query rows of a CTA
+
 // Joins n_parts partial results into `out` (vox_paged.cu).
 cudaError_t launch_paged_merge(PagedType t, const PagedAttnArgs& a, int n_parts, cudaStream_t st);
 
