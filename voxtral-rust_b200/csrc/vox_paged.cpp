@@ -182,10 +182,10 @@ struct KeysPlan {
     int nt = 1, cluster = 1, splits = 1;
 };
 
-// `rows`: query rows of a tile set (a sequence's, or all); `tiles(n)`: tiles of
-// n rows; `keys`: keys that a row can see.
+// `rows`: query rows that share their keys (a sequence's, or all); `all_rows`:
+// tokens x heads; `tiles(n)`: tiles of n rows; `keys`: keys that a row can see.
 template <class F>
-KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t keys, F tiles) {
+KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t all_rows, int64_t keys, F tiles) {
     KeysPlan p;
     const bool fits = c->head_dim == 64 || c->head_dim == 128;
     // tcgen05 tiles have 128 rows: from 32 rows on they win although part of
@@ -193,7 +193,19 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     if (fits && rows > 32 && t != PagedType::F32 && c->page_size >= 8) {
         p.kernel = KeysPlan::TILES;
         const int64_t units = std::max<int64_t>(1, tiles(kPagedTileRows) * (int64_t)c->n_kv_heads);
-        p.splits = (int)std::min<int64_t>(std::max<int64_t>(1, std::min<int64_t>(148 / units, keys / 256)), 64);
+        // The split that ends first: waves of CTAs (one per SM) times a CTA's blocks
+        // of 128 keys, and about 3 blocks' time to start and end one, plus writing
+        // and reading a part of every row (a block takes about 2 us, in which the
+        // memory moves 13 MB).  Many more tiles than SMs even out by themselves
+        // (the longest are first).
+        const int64_t blocks = (keys + 127) / 128;
+        const double part = 8.0 * (double)all_rows * (double)c->head_dim / 13e6;
+        double best = 0;
+        for (int64_t z = 1; z <= std::min<int64_t>(64, std::max<int64_t>(1, blocks / 2)); ++z) {
+            if (z > 1 && units >= 3 * 148) break;
+            const double t = (double)((units * z + 147) / 148) * (double)((blocks + z - 1) / z + 3) + (z > 1 ? part * (double)z : 0.0);
+            if (z == 1 || t < best) best = t, p.splits = (int)z;
+        }
         return p;
     }
     if (fits) p.kernel = KeysPlan::ROWS;
@@ -205,10 +217,10 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     // to 8192 visible keys 411 us against 434 with half as many CTAs.
     const int64_t slots = 148 * (t != PagedType::F32 || p.nt == 1 ? 2 : 1);
     const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (4 * slots + units - 1) / units : 1;
-    // at least 64 keys to a CTA of a cluster (one stream of 1536 tokens: 15 us
-    // through clusters alone, 20 us with a merge behind them), 512 where the
-    // parts go through the merge
-    int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / 64));
+    // At least 64 keys to a CTA of a cluster (one stream of 1536 tokens: 15 us
+    // through clusters alone, 20 us with a merge behind them), 512 where there
+    // are enough tiles without, or where the parts go through the merge.
+    int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / (units < slots ? 64 : 512)));
     if (fits)
         while (p.cluster < 16 && 2 * p.cluster <= parts) p.cluster *= 2;
     parts = std::min<int64_t>(parts / p.cluster, keys / 512 / p.cluster);
@@ -236,12 +248,13 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
     a.n_seqs = (int)b->n_seqs;
     a.max_q = (int)b->max_q_len;
     a.group = (int)group;
-    plan.own = plan_keys(c, t, (int64_t)b->max_q_len * group, visible(b->max_kv_len),
+    const int64_t all_rows = (int64_t)(b->n_tokens * n_heads);
+    plan.own = plan_keys(c, t, (int64_t)b->max_q_len * group, all_rows, visible(b->max_kv_len),
                          [&](int n) { return paged_tiles_bound(a, n); });
     plan.parts = plan.own.splits;
     if (p) {
         a.in_prefix = 1;
-        plan.prefix = plan_keys(c, t, (int64_t)b->n_tokens * group, visible(p->max_len),
+        plan.prefix = plan_keys(c, t, (int64_t)b->n_tokens * group, all_rows, visible(p->max_len),
                                 [&](int n) { return paged_tiles_bound(a, n); });
         plan.parts += plan.prefix.splits;
     }
@@ -326,13 +339,17 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
     const bool aligned = aligned16(a.k, k.type, {a.page_stride, a.head_stride, a.slot_stride}) &&
                          aligned16(a.v, k.type, {}) && aligned16(a.q, k.type, {a.q_ts, a.q_hs}) &&
                          aligned16(a.out, k.type, {a.o_ts, a.o_hs});
+    // The prefix after the sequences' own keys: its launch starts while the other
+    // drains, and waits for it only at its end.
+    a.part0 = plan.prefix.splits * (p != nullptr);
+    TRY(launched(launch_keys(k.type, a, plan.own, aligned, st), "paged attention"));
     if (p) {
         PagedAttnArgs shared = a;
         shared.in_prefix = 1;
+        shared.part0 = 0;
+        shared.follows = 1;
         TRY(launched(launch_keys(k.type, shared, plan.prefix, aligned, st), "prefix attention"));
-        a.part0 = plan.prefix.splits;
     }
-    TRY(launched(launch_keys(k.type, a, plan.own, aligned, st), "paged attention"));
     if (plan.partial) TRY(launched(launch_paged_merge(k.type, a, plan.parts, st), "paged merge"));
     return VOX_OK;
 }

@@ -158,7 +158,11 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     const int h = (blockIdx.x / a.splits) % a.n_kv;
     const int tile = blockIdx.x / a.splits / a.n_kv;
     PagedKeys ks;
-    if (!paged_tile_rows(a, tile, rows, &ks)) return;
+    pdl_allow_dependents();
+    if (!paged_tile_rows(a, tile, rows, &ks)) {
+        pdl_wait_prior_grids();
+        return;
+    }
     for (int i = tid; i < R * hd; i += kGenThreads) {
         const int r = i / hd, d = i % hd;
         float x = 0.f;
@@ -241,15 +245,21 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
                 static_cast<T*>(a.out)[tok * a.o_ts + head * a.o_hs + d] = from_f32<T>(ls == 0.f ? 0.f : acc[r][e] / ls);
         }
     }
+    pdl_wait_prior_grids();  // the launch before this one ends first (PagedAttnArgs::follows)
 }
 
 // ---- joining partial results -----------------------------------------------------
 //
 // out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in the order of the
-// parts.  One warp per (token, head); a part whose sum is 0 is not read.
+// parts; one warp per (token, head).  Bound by reading the parts, and for few
+// rows by latency: a lane takes one part's (m, l), and the parts' results are
+// loaded eight at a time before the first is used.  A part whose sum is 0 is
+// not read.  V: head_dim / 32 where that is 2 or 4 (a lane's elements are then
+// contiguous), 0 for any other.
 
-template <class T>
+template <class T, int V>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a, int n_parts) {
+    constexpr int E = V ? V : kPagedMaxHeadDim / 32;
     const int64_t n_rows = (int64_t)a.n_tokens * a.n_heads;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
@@ -263,27 +273,55 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
     pdl_wait_prior_grids();
     if (!mine) return;
     float top = kNegInf;
-    for (int i = lane; i < n_parts; i += 32) {
-        const float2 ml = a.part_ml[i * n_rows + row];
-        top = fmaxf(top, ml.x);
-    }
+    for (int i = lane; i < n_parts; i += 32) top = fmaxf(top, a.part_ml[i * n_rows + row].x);
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     const float base = top == kNegInf ? 0.f : top;
-    float total = 0.f, acc[kPagedMaxHeadDim / 32] = {};
-    for (int i = 0; i < n_parts; ++i) {
-        const float2 ml = a.part_ml[i * n_rows + row];
-        if (ml.y == 0.f) continue;
-        const float w = exp2f(ml.x - base);
-        total = fmaf(w, ml.y, total);
-        const float* o = a.part_o + (i * n_rows + row) * a.hd;
+    float total = 0.f, acc[E] = {};
+    for (int i0 = 0; i0 < n_parts; i0 += 32) {
+        float w = 0.f, l = 0.f;
+        if (i0 + lane < n_parts) {
+            const float2 ml = a.part_ml[(i0 + lane) * n_rows + row];
+            l = ml.y;
+            w = l == 0.f ? 0.f : exp2f(ml.x - base);
+        }
+        const unsigned used = __ballot_sync(~0u, l != 0.f);
+        const int n = min(32, n_parts - i0);
+        for (int i1 = 0; i1 < n; i1 += 8) {
+            float x[8][E];
 #pragma unroll
-        for (int e = 0; e < kPagedMaxHeadDim / 32; ++e)
-            if (lane + 32 * e < a.hd) acc[e] = fmaf(w, o[lane + 32 * e], acc[e]);
+            for (int i = 0; i < 8; ++i) {
+                const bool take = i1 + i < n && (used >> (i1 + i) & 1);
+                const float* o = a.part_o + ((i0 + i1 + i) * n_rows + row) * a.hd;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+                if (V == 4) {
+                    if (take) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(o + lane * 4);
+                } else if (V == 2) {
+                    if (take) *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(o + lane * 2);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (take && lane + 32 * e < a.hd) x[i][e] = o[lane + 32 * e];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __shfl_sync(~0u, w, (i1 + i) & 31);
+                const float g = __shfl_sync(~0u, l, (i1 + i) & 31);
+                if (i1 + i >= n) break;
+                total = fmaf(f, g, total);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(f, x[i][e], acc[e]);
+            }
+        }
     }
     T* out = static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int e = 0; e < kPagedMaxHeadDim / 32; ++e)
-        if (lane + 32 * e < a.hd) out[lane + 32 * e] = from_f32<T>(total == 0.f ? 0.f : acc[e] / total);
+    for (int e = 0; e < E; ++e) {
+        const int d = V ? lane * V + e : lane + 32 * e;
+        if (V || d < a.hd) out[d] = from_f32<T>(acc[e] * inv);
+    }
 }
 
 template <class F>
@@ -319,8 +357,17 @@ cudaError_t launch_paged_attn_general(PagedType t, const PagedAttnArgs& a, cudaS
             cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) return e;
         }
-        k<<<(unsigned)grid, kGenThreads, smem, st>>>(a);
-        return cudaGetLastError();
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(kGenThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = a.follows ? 1 : 0;
+        return cudaLaunchKernelEx(&cfg, k, a);
     });
 }
 
@@ -336,7 +383,12 @@ cudaError_t launch_paged_merge(PagedType t, const PagedAttnArgs& a, int n_parts,
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return by_type(t, [&](auto x) { return cudaLaunchKernelEx(&cfg, paged_merge_kernel<decltype(x)>, a, n_parts); });
+    return by_type(t, [&](auto x) {
+        using T = decltype(x);
+        if (a.hd == 128) return cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, 4>, a, n_parts);
+        if (a.hd == 64) return cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, 2>, a, n_parts);
+        return cudaLaunchKernelEx(&cfg, paged_merge_kernel<T, 0>, a, n_parts);
+    });
 }
 
 }  // namespace vox

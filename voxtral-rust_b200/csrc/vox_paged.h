@@ -45,6 +45,11 @@ struct PagedAttnArgs {
     float* part_o;
     float2* part_ml;  // (maximum score in log2 units, sum)
     int part0, splits;
+    // 1: the launch may start before the one in front of it in the stream, an
+    // attention kernel over other keys of the same call, has ended (programmatic
+    // dependent launch); it reads nothing of that one and waits for it at its
+    // end, so that whatever waits for this launch has waited for both.
+    int follows;
 };
 
 // Upper bound on the tiles of `rows` query rows, from the host's bounds alone.

@@ -153,43 +153,15 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     // last tiles first: a sequence's later tokens see more keys
     const int tile = (int)(gridDim.x / cs / a.splits / a.n_kv) - 1 - unit / a.splits / a.n_kv;
     PagedKeys ks;
-    if (!paged_tile_rows(a, tile, rows, &ks)) return;  // the whole cluster alike
-
-    // Q^T fragments: one 16-byte word per lane and two k steps (f32: hi and lo of one)
-    {
-        uint32_t* w = reinterpret_cast<uint32_t*>(qf);
-        constexpr int E = 16 / (int)sizeof(T);
-        for (int i = tid; i < ROWS * C; i += kThreads) {
-            const int r = i / C, c = i % C;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (rows.tok[r] >= 0)
-                v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + rows.tok[r] * a.q_ts +
-                                                    (h * a.group + rows.g[r]) * a.q_hs + c * E);
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (F32) {
-                    const int at = (((c >> 1) * NT + (r >> 3)) * 32 + (r & 7) * 4 + j) * 4 + (c & 1);
-                    uint32_t hi, lo;
-                    split_tf32(__uint_as_float(x[j]), hi, lo);
-                    w[at] = hi;
-                    w[at + 2] = lo;
-                } else {
-                    w[(((c >> 2) * NT + (r >> 3)) * 32 + (r & 7) * 4 + j) * 4 + (c & 3)] = x[j];
-                }
-            }
-        }
+    pdl_allow_dependents();
+    if (!paged_tile_rows(a, tile, rows, &ks)) {  // the whole cluster alike
+        pdl_wait_prior_grids();
+        return;
     }
+
     const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 4);
     const int parts = a.splits * cs, part = z * cs + rank;
     const int b0 = (int)((int64_t)kb.total * part / parts), b1 = (int)((int64_t)kb.total * (part + 1) / parts);
-
-    int p[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) p[n][e] = rows.p[n * 8 + 2 * t + e];
-    __syncthreads();
 
     const uint32_t ring = smem_addr(smem) + warp * (U * UNIT);
     const T* const kg = static_cast<const T*>(a.k) + h * a.head_stride;
@@ -242,13 +214,48 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         cp_commit();
     };
 
+    // the first keys and values are on their way before the queries are asked for
+#pragma unroll 1
+    for (int u = 0; u < U - 1; ++u) issue_next();
+
+    // Q^T fragments: one 16-byte word per lane and two k steps (f32: hi and lo of one)
+    {
+        uint32_t* w = reinterpret_cast<uint32_t*>(qf);
+        constexpr int E = 16 / (int)sizeof(T);
+        for (int i = tid; i < ROWS * C; i += kThreads) {
+            const int r = i / C, c = i % C;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (rows.tok[r] >= 0)
+                v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + rows.tok[r] * a.q_ts +
+                                                    (h * a.group + rows.g[r]) * a.q_hs + c * E);
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (F32) {
+                    const int at = (((c >> 1) * NT + (r >> 3)) * 32 + (r & 7) * 4 + j) * 4 + (c & 1);
+                    uint32_t hi, lo;
+                    split_tf32(__uint_as_float(x[j]), hi, lo);
+                    w[at] = hi;
+                    w[at + 2] = lo;
+                } else {
+                    w[(((c >> 2) * NT + (r >> 3)) * 32 + (r & 7) * 4 + j) * 4 + (c & 3)] = x[j];
+                }
+            }
+        }
+    }
+    int p[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) p[n][e] = rows.p[n * 8 + 2 * t + e];
+
+    __syncthreads();
+
     float o[HD / 16][NT][4] = {};
     float m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = kNegInf, l[n][0] = l[n][1] = 0.f;
 
-#pragma unroll 1
-    for (int u = 0; u < U - 1; ++u) issue_next();
     int slot = 0;
     for (int i = b0 + warp; i < b1; i += kWarps) {
         const int j0 = kb.block(i) * kKeys;
@@ -495,6 +502,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         }
     }
     if (cs > 1) cluster.sync();  // the others may still read this CTA's results
+    pdl_wait_prior_grids();      // the launch before this one ends first (PagedAttnArgs::follows)
 }
 
 template <class T, int HD, int NT>
@@ -511,12 +519,14 @@ cudaError_t launch_rows(const PagedAttnArgs& a, int cs, cudaStream_t st) {
     cfg.blockDim = dim3(32 * Cfg::WARPS);
     cfg.dynamicSmemBytes = Cfg::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cs;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cs;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.follows ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, k, a);
 }
 

@@ -13,14 +13,24 @@
 //   warps 0-3  softmax of tile 0: one thread per row
 //   warps 4-7  softmax of tile 1
 //
-// S, P and O stay in tensor memory (S_t 128 columns, its weights P_t in 16 bits
-// over the first 64 of them, O_t up to 128).  The products run in the order
-// P0 V(i), Q0 K(i+1), P1 V(i), Q1 K(i+1): the tensor core executes one thread's
-// products in order, so Q_t K(i+1) may overwrite P_t(i) without a wait.
+// S, P and O stay in tensor memory: O_t up to 128 columns, and for each tile two
+// score buffers of 64 keys, their 16-bit weights over the first 32 columns.  A
+// softmax works on one buffer while the other is filled again:
 //
-// The running maximum of a row moves only when it rises by more than 2^8: until
-// then weights are at most 2^8 (f16 holds 2^15), sums are f32, and O needs no
-// rescaling; the final division by the sum takes any such factor out again.
+//   P_t V(k), then Q_t K(k + 2) into the same columns (one thread's products
+//   execute in order, so no wait lies between the two)
+//
+// What this avoids: with one buffer of 128 keys per tile, a tile's softmax, P V
+// and Q K follow one another, and each hand-over through an mbarrier takes 150 to
+// 250 cycles: 3800 cycles per block of 128 keys against 2048 of products.  The
+// price: at 64 keys (N = 64) Q K reads 6 KB of shared memory per 32 cycles of
+// product and takes 48, so that a block's products are 2560 cycles at D = 128.
+//
+// The running maximum of a row moves only when 64 new weights add up to more
+// than 2^8: until then each is at most 2^8 (f16 holds 2^15), sums are f32, and O
+// needs no rescaling; the final division by the sum takes any such factor out
+// again.  So a step of the common kind costs one FMA, one exponential, one
+// addition and half a conversion per score, and looks for no maximum.
 #include <cuda.h>
 
 #include <type_traits>
@@ -34,7 +44,9 @@ namespace {
 
 constexpr int kTile = 128;  // query rows of a tile, keys of a block
 constexpr int kTileThreads = 320;
-constexpr uint32_t kTmemS = 0, kTmemO = 256, kTmemCols = 512;
+constexpr int kStep = 64;         // keys of a softmax step
+constexpr float kRise = 256.f;    // a step's weights add up to at most this, or the maximum moves
+constexpr uint32_t kTmemO = 0, kTmemS = 256, kTmemCols = 512;  // S_t buffer b at kTmemS + (2 t + b) 64
 
 template <int HD>
 struct TilesCfg {
@@ -49,7 +61,10 @@ struct alignas(64) TileMaps {
     CUtensorMap k, v;
 };
 
-// K-major or MN-major operand in 128-byte-swizzled rows.
+// K-major or MN-major operand in 128-byte-swizzled rows.  Moving on by o bytes
+// adds o >> 4 (the address field is 14 bits, shared memory ends below 2^18): the
+// issuing thread builds a descriptor once per tile, since at 64 cycles a product
+// a dozen instructions in front of each would set the pace.
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
            (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -62,16 +77,59 @@ __host__ __device__ constexpr uint32_t tiles_idesc(bool bf16, int m, int n, bool
            ((uint32_t)(m >> 4) << 24);
 }
 
-// D (TMEM) (+)= A (TMEM) x B (smem)
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// Products and commits of one thread of a converged warp (`leader` is 1 in that
+// thread): predicated, not branched to, so that the warp's descriptors stay in
+// uniform registers.  Behind a branch every product waits for its operands to be
+// moved there, about 110 cycles instead of the 64 it takes to execute.
+__device__ __forceinline__ uint32_t elect_leader() {
+    uint32_t r;
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xFFFFFFFF;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r));
+    return r;
+}
+// D (TMEM) (+)= A (smem) x B (smem)
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
+// D (TMEM) (+)= A (TMEM) x B (smem)
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(leader)
+        : "memory");
+}
+// Waits are bounded by their number of polls (each up to the hardware's own
+// suspension of a few microseconds): no clock is read on the way.
+__device__ __forceinline__ bool tiles_wait(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < (1 << 22); ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
+}
+// A bounded wait of a whole warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tiles_wait(bar, parity)); }
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
                                               uint64_t* bar) {
@@ -94,17 +152,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t ta, uint32_t (&r)[32]) {
         : "r"(ta)
         : "memory");
 }
-// 128 columns: four loads in flight, one wait.
-__device__ __forceinline__ void tmem_ld128(uint32_t ta, uint32_t (&r)[128]) {
+// 64 columns, likewise.
+__device__ __forceinline__ void tmem_ld64(uint32_t ta, uint32_t (&r)[64]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
         "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
-        "}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
-        : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24), R8(r, 32), R8(r, 40), R8(r, 48), R8(r, 56), R8(r, 64), R8(r, 72),
-          R8(r, 80), R8(r, 88), R8(r, 96), R8(r, 104), R8(r, 112), R8(r, 120)
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+        : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24), R8(r, 32), R8(r, 40), R8(r, 48), R8(r, 56)
         : "r"(ta)
         : "memory");
 }
@@ -127,8 +182,77 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t pack_f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Scores of 64 keys that a row does not see become -inf.  p, len, window and
+// sinks are counted from the first of them.
+__device__ __forceinline__ void tiles_mask(uint32_t* s, int p, int len, int window, int sinks) {
+    const int hi = min(p, len - 1), lo = window ? p - window : -1;
+#pragma unroll
+    for (int c = 0; c < 64; ++c)
+        if (c > hi || (c <= lo && c >= sinks)) s[c] = 0xFF800000u;
+}
+
+// Weights 2^(scale s + off) of the 64 scores s, packed into w.  Returns their sum.
+template <class T>
+__device__ __forceinline__ float tiles_weights(const uint32_t* s, uint32_t* w, float scale, float off) {
+    const uint64_t sc = pack_f2(scale, scale), of = pack_f2(off, off);
+#if 1
+    uint64_t sum[2] = {0, 0};
+#else
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#endif
+#pragma unroll
+    for (int c = 0; c < 64; c += 2) {
+        float x, y;
+#if 1
+        unpack_f2(fma_f2(pack_f2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc, of), x, y);
+#else
+        x = fmaf(__uint_as_float(s[c]), scale, off);
+        y = fmaf(__uint_as_float(s[c + 1]), scale, off);
+#endif
+        x = fast_exp2(x);
+        y = fast_exp2(y);
+#if 1
+        sum[(c >> 1) & 1] = add_f2(sum[(c >> 1) & 1], pack_f2(x, y));
+#else
+        sum[c & 3] += x;
+        sum[(c & 3) + 1] += y;
+#endif
+        w[c >> 1] = pack16<T>(x, y);
+    }
+#if 1
+    float s0, s1, s2, s3;
+    unpack_f2(sum[0], s0, s1);
+    unpack_f2(sum[1], s2, s3);
+    return (s0 + s1) + (s2 + s3);
+#else
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#endif
+}
+
 struct TilesShared {
-    uint64_t q_full, kv_full[6], kv_empty[6], s_full[2], p_full[2], pv_done[2], tail;
+    uint64_t q_full, kv_full[6], kv_empty[6], s_full[2][2], p_full[2][2], pv_done[2][2], tail;
     uint32_t tmem;
     int seq, place, pmin, pmax, rows[2], failed;
 };
@@ -144,14 +268,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_sm = base, ring = base + 2 * Cfg::TILE_BYTES;
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
     const int z = blockIdx.x % a.splits, h = (blockIdx.x / a.splits) % a.n_kv;
     const int tile = (int)(gridDim.x / a.splits / a.n_kv) - 1 - blockIdx.x / a.splits / a.n_kv;
 
     // ---- which rows and keys ----
+    pdl_allow_dependents();
     const int plen = a.pfx_len ? paged_prefix_len(a) : 0;
     if (plen < 0) {
         if (tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        pdl_wait_prior_grids();
         return;
     }
     if (tid < 32) {
@@ -166,7 +292,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
     }
     __syncthreads();
-    if (sh.seq < 0) return;
+    if (sh.seq < 0) {
+        pdl_wait_prior_grids();
+        return;
+    }
     PagedKeys ks{a.pfx_pages, plen, a.sinks};
     int tok = -1, p = -1, head = 0;
     if (!a.in_prefix) {
@@ -213,18 +342,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (tid == 0) {
         mbar_init(&sh.q_full, 2 * kTile);
         for (int i = 0; i < U; ++i) mbar_init(&sh.kv_full[i], 1), mbar_init(&sh.kv_empty[i], 1);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i], kTile);
-            mbar_init(&sh.pv_done[i], 1);
-        }
+        for (int t = 0; t < 2; ++t)
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&sh.s_full[t][b], 1);
+                mbar_init(&sh.p_full[t][b], kTile);
+                mbar_init(&sh.pv_done[t][b], 1);
+            }
         mbar_init(&sh.tail, 1);
         fence_barrier_init();
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = __shfl_sync(~0u, sh.tmem, 0);
     const int pmin = sh.pmin, pmax = sh.pmax;
     const bool any = pmin <= pmax;
     const bool two = sh.rows[1];  // rows of tile 1 (tile 0 then has some, or is skipped over as zeros)
@@ -240,7 +370,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         int issued = 0;
         for (int i = 0; i < 2 * n && ok; ++i) {
             const int slot = i % U, blk = kb.block(b0 + (i >> 1));
-            if (i >= U) ok = mbar_wait(&sh.kv_empty[slot], (i / U - 1) & 1);
+            if (i >= U) ok = tiles_wait(&sh.kv_empty[slot], (i / U - 1) & 1);
             ok = __all_sync(~0u, ok);
             if (!ok) break;
             const int j0 = blk * kTile;
@@ -265,7 +395,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             issued = i + 1;
             if (ragged) {
-                ok = __all_sync(~0u, mbar_wait(&sh.tail, 0));
+                ok = __all_sync(~0u, tiles_wait(&sh.tail, 0));
                 if (!ok) break;
                 const int r0 = kb.end - j0, r1 = (r0 + box - 1) & ~(box - 1);
                 for (int e = lane; e < (r1 - r0) * (HD / 8); e += 32) {
@@ -283,76 +413,73 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!ok) {
             // nothing may still be on its way into this CTA's memory when it ends
             if (lane == 0) atomicOr(&sh.failed, 1);
-            for (int i = max(0, issued - U); i < issued; ++i) mbar_wait(&sh.kv_full[i % U], (i / U) & 1);
+            for (int i = max(0, issued - U); i < issued; ++i) tiles_wait(&sh.kv_full[i % U], (i / U) & 1);
         }
     } else if (warp == 8) {
         // ---- products ----
-        constexpr uint32_t id_qk = tiles_idesc(BF16, kTile, kTile, false), id_pv = tiles_idesc(BF16, kTile, HD, true);
-        bool ok = n > 0 && mbar_wait(&sh.q_full, 0);
-        auto wait_kv = [&](int i) { return mbar_wait(&sh.kv_full[i % U], (i / U) & 1); };
-        auto qk = [&](int t, int i) {
-            if (lane == 0) {
-                const uint32_t k0 = ring + ((2 * i) % U) * Cfg::TILE_BYTES, q0 = q_sm + t * Cfg::TILE_BYTES;
+        constexpr uint32_t id_qk = tiles_idesc(BF16, kTile, kStep, false), id_pv = tiles_idesc(BF16, kTile, HD, true);
+        const uint32_t leader = elect_leader();
+        bool ok = n > 0 && warp_wait(&sh.q_full, 0);
+        auto wait_kv = [&](int i) { return warp_wait(&sh.kv_full[i % U], (i / U) & 1); };
+        const uint64_t q_desc = sw128_desc(q_sm, 16, 1024), k_desc = sw128_desc(ring, 16, 1024),
+                       v_desc = sw128_desc(ring, Cfg::HALF, 1024);
+        // step k is half k & 1 of block k / 2
+        auto qk = [&](int t, int half, uint64_t kd) {
+            const uint64_t qd = q_desc + t * (Cfg::TILE_BYTES >> 4);
+            const uint32_t d = tmem + kTmemS + (2 * t + half) * kStep;
 #pragma unroll
-                for (int x = 0; x < HD / 16; ++x) {
-                    const uint32_t o = (x >> 2) * Cfg::HALF + (x & 3) * 32;
-                    umma_f16(tmem + kTmemS + t * kTile, sw128_desc(q0 + o, 16, 1024), sw128_desc(k0 + o, 16, 1024), id_qk, x > 0);
-                }
-                umma_commit(&sh.s_full[t]);
+            for (int x = 0; x < HD / 16; ++x) {
+                const uint32_t o = ((x >> 2) * Cfg::HALF + (x & 3) * 32) >> 4;
+                umma_ss(leader, d, qd + o, kd + half * (kStep * 128 >> 4) + o, id_qk, x > 0);
             }
-            __syncwarp();
+            umma_commit_if(leader, &sh.s_full[t][half]);
         };
-        auto pv = [&](int t, int i) {
-            if (lane == 0) {
-                const uint32_t v0 = ring + ((2 * i + 1) % U) * Cfg::TILE_BYTES;
+        auto pv = [&](int t, int half, uint64_t vd, uint32_t more) {
+            const uint32_t d = tmem + kTmemO + t * HD, pt = tmem + kTmemS + (2 * t + half) * kStep;
 #pragma unroll
-                for (int x = 0; x < kTile / 16; ++x)
-                    umma_f16_ts(tmem + kTmemO + t * HD, tmem + kTmemS + t * kTile + x * 8, sw128_desc(v0 + x * 2048, Cfg::HALF, 1024),
-                                id_pv, i > 0 || x > 0);
-                umma_commit(&sh.pv_done[t]);
-            }
-            __syncwarp();
+            for (int x = 0; x < kStep / 16; ++x)
+                umma_ts(leader, d, pt + x * 8, vd + (((half * kStep + x * 16) * 128) >> 4), id_pv, x > 0 ? 1u : more);
+            umma_commit_if(leader, &sh.pv_done[t][half]);
         };
+        auto unit = [&](uint64_t desc, int i) { return desc + (i % U) * (Cfg::TILE_BYTES >> 4); };
+        // only where a later tile waits for it: no arrival may outlive the CTA
         auto free_unit = [&](int i) {
-            // only where a later tile waits for it: no arrival may outlive the CTA
-            if (lane == 0 && i + U < 2 * n) umma_commit(&sh.kv_empty[i % U]);
-            __syncwarp();
+            if (i + U < 2 * n) umma_commit_if(leader, &sh.kv_empty[i % U]);
         };
         if (ok && (ok = wait_kv(0))) {
             tmem_fence_after();
-            qk(0, 0);
-            if (two) qk(1, 0);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                qk(0, half, k_desc);
+                if (two) qk(1, half, k_desc);
+            }
             free_unit(0);
         }
+#pragma unroll 1
         for (int i = 0; i < n && ok; ++i) {
-            const bool more = i + 1 < n;
-            ok = wait_kv(2 * i + 1) && mbar_wait(&sh.p_full[0], i & 1);
-            if (!ok) break;
-            tmem_fence_after();
-            pv(0, i);
-            if (more) {
-                ok = wait_kv(2 * i + 2);
-                if (!ok) break;
-                qk(0, i + 1);
-            }
-            if (two) {
-                ok = mbar_wait(&sh.p_full[1], i & 1);
-                if (!ok) break;
-                tmem_fence_after();
-                pv(1, i);
-            }
+            const bool next = i + 1 < n;
+            const uint64_t vd = unit(v_desc, 2 * i + 1), kd = unit(k_desc, 2 * i + 2);
+            ok = wait_kv(2 * i + 1) && (!next || wait_kv(2 * i + 2));
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t && !two) continue;
+                    ok = ok && warp_wait(&sh.p_full[t][half], i & 1);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    pv(t, half, vd, i > 0 || half > 0);
+                    if (next) qk(t, half, kd);
+                }
             free_unit(2 * i + 1);
-            if (more) {
-                if (two) qk(1, i + 1);
-                free_unit(2 * i + 2);
-            }
+            free_unit(2 * i + 2);
         }
         if (!ok && n > 0 && lane == 0) atomicOr(&sh.failed, 1);
     } else {
         // ---- softmax ----
         const int t = warp >> 2, r = tid & (kTile - 1);
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const uint32_t t_s = tmem + kTmemS + t * kTile + lanes, t_o = tmem + kTmemO + t * HD + lanes;
+        const uint32_t t_s = tmem + kTmemS + t * (2 * kStep) + lanes, t_o = tmem + kTmemO + t * HD + lanes;
         {
             const uint32_t dst = q_sm + t * Cfg::TILE_BYTES + r * 128;
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (tok >= 0 ? tok * a.q_ts + head * a.q_hs : 0));
@@ -367,68 +494,56 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(&sh.q_full);
         }
-        float m = kNegInf, l = 0.f;
+        float m = tok >= 0 ? kNegInf : 0.f, l = 0.f;
         bool ok = true;
-        const int steps = t == 0 || two ? n : 0;
-        for (int i = 0; i < steps; ++i) {
-            ok = mbar_wait(&sh.s_full[t], i & 1);
-            if (!__all_sync(~0u, ok)) break;
-            tmem_fence_after();
-            uint32_t s[kTile];
-            tmem_ld128(t_s, s);
-            const int j0 = kb.block(b0 + i) * kTile;
-            const bool all = j0 + kTile - 1 <= pmin && j0 + kTile <= ks.len &&
-                             (a.window == 0 || j0 > pmax - a.window || j0 + kTile <= ks.sinks);
-            if (!all) {
-#pragma unroll
-                for (int c = 0; c < kTile; ++c)
-                    if (!paged_sees(p, j0 + c, ks.len, a.window, ks.sinks)) s[c] = 0xFF800000u;
-            }
-            float top[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-#pragma unroll
-            for (int c = 0; c < kTile; c += 8)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    top[e] = fmaxf(fmaxf(top[e], __uint_as_float(s[c + 2 * e])), __uint_as_float(s[c + 2 * e + 1]));
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
-            const bool rise = mx > m + 8.f;
-            if (i == 0) {
-                m = mx;
-            } else if (__any_sync(~0u, rise)) {
-                const float m_new = rise ? mx : m;
-                const float f = m_new == kNegInf ? 1.f : fast_exp2(m - m_new);
-                l *= f;
-                m = m_new;
-                ok = mbar_wait(&sh.pv_done[t], (i - 1) & 1);
-                if (!__all_sync(~0u, ok)) break;
-                tmem_fence_after();
+        const int steps = t == 0 || two ? 2 * n : 0;
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(t_o + c, o);
+        for (int k = 0; k < steps; ++k) {
+            ok = __all_sync(~0u, tiles_wait(&sh.s_full[t][k & 1], (k >> 1) & 1));
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t buf = t_s + (k & 1) * kStep;
+            uint32_t s[kStep], w[kStep / 2];
+            const int j0 = kb.block(b0 + (k >> 1)) * kTile + (k & 1) * kStep;
+            const bool all = j0 + kStep - 1 <= pmin && j0 + kStep <= ks.len &&
+                             (a.window == 0 || j0 > pmax - a.window || j0 + kStep <= ks.sinks);
+            tmem_ld64(buf, s);
+            if (!all) tiles_mask(s, p - j0, ks.len - j0, a.window, ks.sinks - j0);
+            // The weights are taken with the maximum so far.  Only where their sum says
+            // that a score may have risen far above it (the first steps, mostly) is the
+            // new maximum looked for and the weights taken again.
+            float l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
+            if (__any_sync(~0u, l_new > kRise || m == kNegInf)) {
+                float mx = kNegInf;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tmem_st32(t_o + c, o);
+                for (int c = 0; c < kStep; c += 2) mx = max3(mx, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                const float m_new = fmaxf(m, mx * a.scale_log2);
+                const float f = m_new == kNegInf ? 1.f : fast_exp2(m - m_new);
+                m = m_new;
+                l *= f;
+                if (k > 0) {
+                    ok = __all_sync(~0u, tiles_wait(&sh.pv_done[t][(k - 1) & 1], ((k - 1) >> 1) & 1));
+                    if (!ok) break;
+                    tmem_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + c, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(t_o + c, o);
+                    }
                 }
+                l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
             }
-            const float off = m == kNegInf ? 0.f : -m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < kTile; c += 2) {
-                const float x = fast_exp2(fmaf(__uint_as_float(s[c]), a.scale_log2, off));
-                const float y = fast_exp2(fmaf(__uint_as_float(s[c + 1]), a.scale_log2, off));
-                sum[(c >> 1) & 3] += x + y;
-                s[c >> 1] = pack16<T>(x, y);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st32(t_s, s);
-            tmem_st32(t_s + 32, s + 32);
+            l += l_new;
+            tmem_st32(buf, w);
             tmem_wait_st();
             tmem_fence_before();
-            mbar_arrive(&sh.p_full[t]);
+            mbar_arrive(&sh.p_full[t][k & 1]);
         }
         // ---- the result ----
-        if (ok && steps > 0) ok = mbar_wait(&sh.pv_done[t], (steps - 1) & 1);
+        if (ok && steps > 0) ok = tiles_wait(&sh.pv_done[t][1], (n - 1) & 1);
         ok = __all_sync(~0u, ok);
         if (!ok && lane == 0) atomicOr(&sh.failed, 1);
         tmem_fence_after();
@@ -497,13 +612,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mbar_init(&sh.q_full, 1);
                 fence_barrier_init();
                 umma_commit(&sh.q_full);
-                mbar_wait(&sh.q_full, 0);
+                tiles_wait(&sh.q_full, 0);
             }
             __syncwarp();
         }
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
     }
+    pdl_wait_prior_grids();  // the launch before this one ends first (PagedAttnArgs::follows)
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -529,8 +645,17 @@ cudaError_t launch_tiles(const PagedAttnArgs& a, const TileMaps& maps, cudaStrea
     if (e != cudaSuccess) return e;
     const int64_t grid = paged_tiles_bound(a, 2 * kTile) * a.n_kv * a.splits;
     if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    k<<<(unsigned)grid, kTileThreads, TilesCfg<HD>::SMEM, st>>>(a, maps);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = TilesCfg<HD>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = a.follows ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k, a, maps);
 }
 
 }  // namespace
