@@ -8,10 +8,12 @@
 // that share every K and V tile, so that one tile's softmax runs while the
 // other's products do:
 //
-//   warp 9     K and V tiles of 128 keys from their pages, TMA into a ring
-//   warp 8     S_t = Q_t K^T and O_t += P_t V, one thread issuing tcgen05.mma
-//   warps 0-3  softmax of tile 0: one thread per row
-//   warps 4-7  softmax of tile 1
+//   warp 10      K and V tiles of 128 keys from their pages, TMA into a ring
+//   warps 8, 9   S_t = Q_t K^T and O_t += P_t V of tile 0 and 1, one thread each
+//                issuing tcgen05.mma (from one thread for both, a tile's products
+//                wait behind the other tile's softmax)
+//   warps 0-3    softmax of tile 0: one thread per row
+//   warps 4-7    softmax of tile 1
 //
 // S, P and O stay in tensor memory: O_t up to 128 columns, and for each tile two
 // score buffers of 64 keys, their 16-bit weights over the first 32 columns.  A
@@ -43,7 +45,7 @@ namespace vox {
 namespace {
 
 constexpr int kTile = 128;  // query rows of a tile, keys of a block
-constexpr int kTileThreads = 320;
+constexpr int kTileThreads = 352;
 constexpr int kStep = 64;         // keys of a softmax step
 constexpr float kRise = 256.f;    // a step's weights add up to at most this, or the maximum moves
 constexpr uint32_t kTmemO = 0, kTmemS = 256, kTmemCols = 512;  // S_t buffer b at kTmemS + (2 t + b) 64
@@ -213,46 +215,41 @@ __device__ __forceinline__ void tiles_mask(uint32_t* s, int p, int len, int wind
         if (c > hi || (c <= lo && c >= sinks)) s[c] = 0xFF800000u;
 }
 
-// Weights 2^(scale s + off) of the 64 scores s, packed into w.  Returns their sum.
+// Weights 2^(scale s + off) of the 64 scores s, packed into w.  Returns their
+// sum.  In groups of G: a group's exponentials go out before the last group's
+// results are used, so that their latency is covered without a second warp.
 template <class T>
 __device__ __forceinline__ float tiles_weights(const uint32_t* s, uint32_t* w, float scale, float off) {
+    constexpr int G = 16, N = 64 / G;
     const uint64_t sc = pack_f2(scale, scale), of = pack_f2(off, off);
-#if 1
     uint64_t sum[2] = {0, 0};
-#else
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#endif
+    float x[N][G];
 #pragma unroll
-    for (int c = 0; c < 64; c += 2) {
-        float x, y;
-#if 1
-        unpack_f2(fma_f2(pack_f2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc, of), x, y);
-#else
-        x = fmaf(__uint_as_float(s[c]), scale, off);
-        y = fmaf(__uint_as_float(s[c + 1]), scale, off);
-#endif
-        x = fast_exp2(x);
-        y = fast_exp2(y);
-#if 1
-        sum[(c >> 1) & 1] = add_f2(sum[(c >> 1) & 1], pack_f2(x, y));
-#else
-        sum[c & 3] += x;
-        sum[(c & 3) + 1] += y;
-#endif
-        w[c >> 1] = pack16<T>(x, y);
+    for (int g = 0; g <= N; ++g) {
+        if (g < N) {
+#pragma unroll
+            for (int c = 0; c < G; c += 2)
+                unpack_f2(fma_f2(pack_f2(__uint_as_float(s[g * G + c]), __uint_as_float(s[g * G + c + 1])), sc, of), x[g][c], x[g][c + 1]);
+#pragma unroll
+            for (int c = 0; c < G; ++c) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[g][c]));
+        }
+        if (g > 0) {
+#pragma unroll
+            for (int c = 0; c < G; c += 2) {
+                const float a = x[g - 1][c], b = x[g - 1][c + 1];
+                sum[(c >> 1) & 1] = add_f2(sum[(c >> 1) & 1], pack_f2(a, b));
+                w[((g - 1) * G + c) >> 1] = pack16<T>(a, b);
+            }
+        }
     }
-#if 1
     float s0, s1, s2, s3;
     unpack_f2(sum[0], s0, s1);
     unpack_f2(sum[1], s2, s3);
     return (s0 + s1) + (s2 + s3);
-#else
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#endif
 }
 
 struct TilesShared {
-    uint64_t q_full, kv_full[6], kv_empty[6], s_full[2][2], p_full[2][2], pv_done[2][2], tail;
+    uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2][2], p_full[2][2], pv_done[2][2], tail;
     uint32_t tmem;
     int seq, place, pmin, pmax, rows[2], failed;
 };
@@ -340,12 +337,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     if (tid == 0) {
-        mbar_init(&sh.q_full, 2 * kTile);
-        for (int i = 0; i < U; ++i) mbar_init(&sh.kv_full[i], 1), mbar_init(&sh.kv_empty[i], 1);
+        mbar_init(&sh.q_full[0], kTile);
+        mbar_init(&sh.q_full[1], kTile);
+        for (int i = 0; i < U; ++i) mbar_init(&sh.kv_full[i], 1), mbar_init(&sh.kv_empty[i], 2);  // both tiles are done with it
         for (int t = 0; t < 2; ++t)
             for (int b = 0; b < 2; ++b) {
                 mbar_init(&sh.s_full[t][b], 1);
-                mbar_init(&sh.p_full[t][b], kTile);
+                mbar_init(&sh.p_full[t][b], 4);  // one arrival a warp
                 mbar_init(&sh.pv_done[t][b], 1);
             }
         mbar_init(&sh.tail, 1);
@@ -362,7 +360,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int b0 = any ? (int)((int64_t)kb.total * z / a.splits) : 0;
     const int n = any ? (int)((int64_t)kb.total * (z + 1) / a.splits) - b0 : 0;
 
-    if (warp == 9) {
+    if (warp == 10) {
         // ---- K and V tiles ----
         const int ps = 1 << a.page_shift;
         const int box = min(ps, kTile), boxes = kTile / box;
@@ -415,66 +413,61 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (lane == 0) atomicOr(&sh.failed, 1);
             for (int i = max(0, issued - U); i < issued; ++i) tiles_wait(&sh.kv_full[i % U], (i / U) & 1);
         }
-    } else if (warp == 8) {
-        // ---- products ----
+    } else if (warp >= 8) {
+        // ---- products of tile t ----
+        const int t = warp - 8, steps = t == 0 || two ? n : 0;
         constexpr uint32_t id_qk = tiles_idesc(BF16, kTile, kStep, false), id_pv = tiles_idesc(BF16, kTile, HD, true);
         const uint32_t leader = elect_leader();
-        bool ok = n > 0 && warp_wait(&sh.q_full, 0);
+        bool ok = steps > 0 && warp_wait(&sh.q_full[t], 0);
         auto wait_kv = [&](int i) { return warp_wait(&sh.kv_full[i % U], (i / U) & 1); };
         const uint64_t q_desc = sw128_desc(q_sm, 16, 1024), k_desc = sw128_desc(ring, 16, 1024),
                        v_desc = sw128_desc(ring, Cfg::HALF, 1024);
-        // step k is half k & 1 of block k / 2
-        auto qk = [&](int t, int half, uint64_t kd) {
-            const uint64_t qd = q_desc + t * (Cfg::TILE_BYTES >> 4);
-            const uint32_t d = tmem + kTmemS + (2 * t + half) * kStep;
+        const uint64_t qd = q_desc + t * (Cfg::TILE_BYTES >> 4);
+        const uint32_t t_o = tmem + kTmemO + t * HD, t_s = tmem + kTmemS + t * (2 * kStep);
+        auto qk = [&](int half, uint64_t kd) {
 #pragma unroll
             for (int x = 0; x < HD / 16; ++x) {
                 const uint32_t o = ((x >> 2) * Cfg::HALF + (x & 3) * 32) >> 4;
-                umma_ss(leader, d, qd + o, kd + half * (kStep * 128 >> 4) + o, id_qk, x > 0);
+                umma_ss(leader, t_s + half * kStep, qd + o, kd + half * (kStep * 128 >> 4) + o, id_qk, x > 0);
             }
             umma_commit_if(leader, &sh.s_full[t][half]);
         };
-        auto pv = [&](int t, int half, uint64_t vd, uint32_t more) {
-            const uint32_t d = tmem + kTmemO + t * HD, pt = tmem + kTmemS + (2 * t + half) * kStep;
+        auto pv = [&](int half, uint64_t vd, uint32_t more) {
 #pragma unroll
             for (int x = 0; x < kStep / 16; ++x)
-                umma_ts(leader, d, pt + x * 8, vd + (((half * kStep + x * 16) * 128) >> 4), id_pv, x > 0 ? 1u : more);
+                umma_ts(leader, t_o, t_s + half * kStep + x * 8, vd + (((half * kStep + x * 16) * 128) >> 4), id_pv, x > 0 ? 1u : more);
             umma_commit_if(leader, &sh.pv_done[t][half]);
         };
         auto unit = [&](uint64_t desc, int i) { return desc + (i % U) * (Cfg::TILE_BYTES >> 4); };
         // only where a later tile waits for it: no arrival may outlive the CTA
         auto free_unit = [&](int i) {
-            if (i + U < 2 * n) umma_commit_if(leader, &sh.kv_empty[i % U]);
+            if (i + U >= 2 * n) return;
+            umma_commit_if(leader, &sh.kv_empty[i % U]);
+            if (!two) umma_commit_if(leader, &sh.kv_empty[i % U]);
         };
         if (ok && (ok = wait_kv(0))) {
             tmem_fence_after();
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                qk(0, half, k_desc);
-                if (two) qk(1, half, k_desc);
-            }
+            qk(0, k_desc);
+            qk(1, k_desc);
             free_unit(0);
         }
 #pragma unroll 1
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < steps && ok; ++i) {
             const bool next = i + 1 < n;
             const uint64_t vd = unit(v_desc, 2 * i + 1), kd = unit(k_desc, 2 * i + 2);
             ok = wait_kv(2 * i + 1) && (!next || wait_kv(2 * i + 2));
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (t && !two) continue;
-                    ok = ok && warp_wait(&sh.p_full[t][half], i & 1);
-                    if (!ok) break;
-                    tmem_fence_after();
-                    pv(t, half, vd, i > 0 || half > 0);
-                    if (next) qk(t, half, kd);
-                }
+            for (int half = 0; half < 2; ++half) {
+                ok = ok && warp_wait(&sh.p_full[t][half], i & 1);
+                if (!ok) break;
+                tmem_fence_after();
+                pv(half, vd, i > 0 || half > 0);
+                if (next) qk(half, kd);
+            }
             free_unit(2 * i + 1);
             free_unit(2 * i + 2);
         }
-        if (!ok && n > 0 && lane == 0) atomicOr(&sh.failed, 1);
+        if (!ok && steps > 0 && lane == 0) atomicOr(&sh.failed, 1);
     } else {
         // ---- softmax ----
         const int t = warp >> 2, r = tid & (kTile - 1);
@@ -492,7 +485,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                              "r"(v[c].x), "r"(v[c].y), "r"(v[c].z), "r"(v[c].w)
                              : "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&sh.q_full);
+            mbar_arrive(&sh.q_full[t]);
         }
         float m = tok >= 0 ? kNegInf : 0.f, l = 0.f;
         bool ok = true;
@@ -540,7 +533,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             tmem_st32(buf, w);
             tmem_wait_st();
             tmem_fence_before();
-            mbar_arrive(&sh.p_full[t][k & 1]);
+            __syncwarp();
+            // 128 arrivals on one barrier would queue up for about 200 cycles
+            if (lane == 0) mbar_arrive(&sh.p_full[t][k & 1]);
         }
         // ---- the result ----
         if (ok && steps > 0) ok = tiles_wait(&sh.pv_done[t][1], (n - 1) & 1);
@@ -604,18 +599,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_fence_before();
     }
     __syncthreads();
-    if (warp == 8) {
-        if (sh.failed) {
-            // products may be in flight: let them end before their memory goes
-            if (lane == 0) {
-                paged_status(a, VOX_PAGED_TIMEOUT);
-                mbar_init(&sh.q_full, 1);
-                fence_barrier_init();
-                umma_commit(&sh.q_full);
-                tiles_wait(&sh.q_full, 0);
-            }
-            __syncwarp();
+    if (sh.failed) {
+        // products may be in flight: let them end before their memory goes
+        if (warp >= 8 && warp < 10 && lane == 0) {
+            paged_status(a, VOX_PAGED_TIMEOUT);
+            mbar_init(&sh.q_full[warp - 8], 1);
+            fence_barrier_init();
+            umma_commit(&sh.q_full[warp - 8]);
+            tiles_wait(&sh.q_full[warp - 8], 0);
         }
+        __syncthreads();
+    }
+    if (warp == 8) {
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
     }
