@@ -251,7 +251,8 @@ __device__ __forceinline__ float tiles_weights(const uint32_t* s, uint32_t* w, f
 struct TilesShared {
     uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2][2], p_full[2][2], pv_done[2][2], tail;
     uint32_t tmem;
-    int seq, place, pmin, pmax, rows[2], failed;
+    int lo[8], hi[8];  // smallest and largest index of a warp's rows
+    int failed;
 };
 
 template <class T, int HD>
@@ -277,31 +278,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         pdl_wait_prior_grids();
         return;
     }
-    if (tid < 32) {
-        int place = tile, s = 0;
-        if (!a.in_prefix) s = paged_find_tile(a, tile, 2 * kTile, &place);
-        if (tid == 0) {
-            sh.seq = s;
-            sh.place = place;
-            sh.pmin = 0x7FFFFFFF;
-            sh.pmax = -0x7FFFFFFF;
-            sh.rows[0] = sh.rows[1] = sh.failed = 0;
-        }
-    }
-    __syncthreads();
-    if (sh.seq < 0) {
+    // every warp looks for itself: one block-wide barrier in the whole prologue
+    int place = tile, seq = 0;
+    if (!a.in_prefix) seq = paged_find_tile(a, tile, 2 * kTile, &place);
+    if (seq < 0) {
         pdl_wait_prior_grids();
         return;
     }
     PagedKeys ks{a.pfx_pages, plen, a.sinks};
     int tok = -1, p = -1, head = 0;
     if (!a.in_prefix) {
-        const PagedSeq q = paged_seq(a, sh.seq);
+        const PagedSeq q = paged_seq(a, seq);
         if (!q.ok && tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
-        ks.table = a.table + sh.seq * a.table_stride;
+        ks.table = a.table + seq * a.table_stride;
         ks.len = q.len;
         ks.sinks = max(0, a.sinks - plen);
-        const int64_t row = (int64_t)sh.place * (2 * kTile) + tid;
+        const int64_t row = (int64_t)place * (2 * kTile) + tid;
         if (tid < 2 * kTile && row < (int64_t)q.nq * a.group) {
             const int i = (int)(row / a.group);
             tok = q.q0 + i;
@@ -323,22 +315,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         }
     }
-    {
+    // The queries are asked for before anything is set up: a warp's 32 rows, each
+    // 16-byte column by a lane (a thread reading its own row would touch 32 lines
+    // at a time: 7000 cycles instead of 2000).
+    constexpr int QC = HD / 8, QR = 32 / QC;  // columns of a row, rows at once
+    uint4 qv[32 / QR];
+    if (warp < 8) {
+#pragma unroll
+        for (int i = 0; i < 32 / QR; ++i) {
+            const int r = i * QR + lane / QC;
+            const int rt = __shfl_sync(~0u, tok, r), rh = __shfl_sync(~0u, head, r);
+            qv[i] = make_uint4(0, 0, 0, 0);
+            if (rt >= 0)
+                qv[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + rt * a.q_ts + rh * a.q_hs + (lane % QC) * 8);
+        }
         const int lo = __reduce_min_sync(~0u, tok >= 0 ? p : 0x7FFFFFFF);
         const int hi = __reduce_max_sync(~0u, tok >= 0 ? p : -0x7FFFFFFF);
-        if (lane == 0 && lo <= hi) {
-            atomicMin(&sh.pmin, lo);
-            atomicMax(&sh.pmax, hi);
-            sh.rows[warp >> 2] = 1;
-        }
+        if (lane == 0) sh.lo[warp] = lo, sh.hi[warp] = hi;
     }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "r"(kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (tid == 0) {
-        mbar_init(&sh.q_full[0], kTile);
-        mbar_init(&sh.q_full[1], kTile);
+    if (tid == 10 * 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+        sh.failed = 0;
+        mbar_init(&sh.q_full[0], 4);  // one arrival a warp
+        mbar_init(&sh.q_full[1], 4);
         for (int i = 0; i < U; ++i) mbar_init(&sh.kv_full[i], 1), mbar_init(&sh.kv_empty[i], 2);  // both tiles are done with it
         for (int t = 0; t < 2; ++t)
             for (int b = 0; b < 2; ++b) {
@@ -353,9 +357,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(~0u, sh.tmem, 0);
-    const int pmin = sh.pmin, pmax = sh.pmax;
+    int pmin = 0x7FFFFFFF, pmax = -0x7FFFFFFF;
+    bool two = false;  // tile 1 has rows (tile 0 then has some, or counts as zeros)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        pmin = min(pmin, sh.lo[i]);
+        pmax = max(pmax, sh.hi[i]);
+        two |= i >= 4 && sh.lo[i] <= sh.hi[i];
+    }
     const bool any = pmin <= pmax;
-    const bool two = sh.rows[1];  // rows of tile 1 (tile 0 then has some, or is skipped over as zeros)
     const KeyBlocks kb = paged_key_blocks(pmin, pmax, ks.len, a.window, ks.sinks, 7);
     const int b0 = any ? (int)((int64_t)kb.total * z / a.splits) : 0;
     const int n = any ? (int)((int64_t)kb.total * (z + 1) / a.splits) - b0 : 0;
@@ -470,23 +480,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!ok && steps > 0 && lane == 0) atomicOr(&sh.failed, 1);
     } else {
         // ---- softmax ----
-        const int t = warp >> 2, r = tid & (kTile - 1);
+        const int t = warp >> 2;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t t_s = tmem + kTmemS + t * (2 * kStep) + lanes, t_o = tmem + kTmemO + t * HD + lanes;
-        {
-            const uint32_t dst = q_sm + t * Cfg::TILE_BYTES + r * 128;
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (tok >= 0 ? tok * a.q_ts + head * a.q_hs : 0));
-            uint4 v[HD / 8];
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) v[c] = tok >= 0 ? src[c] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c)
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * Cfg::HALF + (((c & 7) ^ (r & 7)) << 4)),
-                             "r"(v[c].x), "r"(v[c].y), "r"(v[c].z), "r"(v[c].w)
-                             : "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&sh.q_full[t]);
+        for (int i = 0; i < 32 / QR; ++i) {
+            const int r = (warp & 3) * 32 + i * QR + lane / QC, c = lane % QC;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_sm + t * Cfg::TILE_BYTES + (c >> 3) * Cfg::HALF +
+                                                                         r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                         "r"(qv[i].x), "r"(qv[i].y), "r"(qv[i].z), "r"(qv[i].w)
+                         : "memory");
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full[t]);
         float m = tok >= 0 ? kNegInf : 0.f, l = 0.f;
         bool ok = true;
         const int steps = t == 0 || two ? 2 * n : 0;
@@ -505,8 +512,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             // The weights are taken with the maximum so far.  Only where their sum says
             // that a score may have risen far above it (the first steps, mostly) is the
             // new maximum looked for and the weights taken again.
-            float l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
-            if (__any_sync(~0u, l_new > kRise || m == kNegInf)) {
+            float l_new = 0.f;
+            if (k > 0) l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
+            if (k == 0 || __any_sync(~0u, l_new > kRise || m == kNegInf)) {
                 float mx = kNegInf;
 #pragma unroll
                 for (int c = 0; c < kStep; c += 2) mx = max3(mx, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
@@ -547,40 +555,65 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (a.part_o && write) a.part_ml[at] = make_float2(m, l);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bool odd = false;
+        // The rows go through the tile's queries' memory (all products with them are
+        // done), 32 floats or 64 results of a row at a time, so that a store covers
+        // 128 bytes of a row; the 16-byte columns are swizzled by the row.
+        const uint32_t stage = q_sm + t * Cfg::TILE_BYTES + (warp & 3) * (32 * 128);
+        const int64_t row_at = a.part_o ? at * HD : tok * a.o_ts + head * a.o_hs;
+        const int width = a.part_o ? 32 : 64;  // elements of 128 bytes
         if (ok) {
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t o[32];
-                if (steps > 0) {
-                    tmem_ld32(t_o + c, o);
-                } else {
+            for (int c0 = 0; c0 < HD; c0 += width) {
+#pragma unroll 1
+                for (int c = c0; c < c0 + width; c += 32) {
+                    uint32_t o[32];
+                    if (steps > 0) {
+                        tmem_ld32(t_o + c, o);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0u;
-                }
-                float check = 0.f;
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
+                    }
+                    float check = 0.f;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) check += fabsf(__uint_as_float(o[e]));
-                odd |= !(check < __builtin_huge_valf());
-                if (!write) continue;
-                if (a.part_o) {
-                    float4* dst = reinterpret_cast<float4*>(a.part_o + at * HD + c);
+                    for (int e = 0; e < 32; ++e) check += fabsf(__uint_as_float(o[e]));
+                    odd |= !(check < __builtin_huge_valf());
+                    if (!a.part_o) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            o[e] = pack16<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                             __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-                } else {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + c);
-                    uint32_t w[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        w[e] = pack16<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dst[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                        if (a.part_o || e < 4)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 +
+                                                                                         ((((c - c0) / 8 + e) ^ (lane & 7)) << 4)),
+                                         "r"(o[4 * e]), "r"(o[4 * e + 1]), "r"(o[4 * e + 2]), "r"(o[4 * e + 3])
+                                         : "memory");
                 }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * 4 + lane / 8, e = lane % 8;
+                    const int64_t ra = __shfl_sync(~0u, row_at, r);
+                    const bool rw = __shfl_sync(~0u, write, r);
+                    uint4 v;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(stage + r * 128 + ((e ^ (r & 7)) << 4))
+                                 : "memory");
+                    if (rw) {
+                        if (a.part_o)
+                            *reinterpret_cast<uint4*>(a.part_o + ra + c0 + e * 4) = v;
+                        else
+                            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ra + c0 + e * 8) = v;
+                    }
+                }
+                __syncwarp();
             }
         }
         // A value that is not finite may have come from a key that the row does
         // not see (0 x inf): such rows are done again key by key.
+        __syncwarp();
         for (unsigned todo = __ballot_sync(~0u, odd && write); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const int rt = __shfl_sync(~0u, tok, src), rh = __shfl_sync(~0u, head, src), rp = __shfl_sync(~0u, p, src);
