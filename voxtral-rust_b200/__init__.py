@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import weakref
 
 import numpy as np
@@ -1137,7 +1138,13 @@ def softmax_inplace(ctx: Context, x):
 # outputs come from torch's allocator, so calls on several streams and in
 # several captured graphs do not share any.
 
+# A call costs the host little more than its launches: descriptors of one call
+# are packed bytes (the layout of Rows and PagedPrefixDesc).
+
 _paged_dtypes = None
+_paged_torch = None   # (torch, current raw stream of a device index)
+_pack_rows = struct.Struct("PNN").pack
+_pack_prefix = struct.Struct("PPNN").pack
 
 
 def _paged_dtype(t, name):
@@ -1151,9 +1158,13 @@ def _paged_dtype(t, name):
     return _paged_dtypes[t.dtype]
 
 
-def _paged_stream(device):
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+def _paged_env():
+    global _paged_torch
+    if _paged_torch is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _paged_torch = (torch, raw or (lambda index: torch.cuda.current_stream(index).cuda_stream), lib())
+    return _paged_torch
 
 
 class PagedKvCache:
@@ -1178,7 +1189,7 @@ class PagedKvCache:
         head = head if self.n_kv_heads > 1 else max(slot, self.head_dim)
         page = page if self.n_pages > 1 else max(head, slot, self.head_dim)
         self.k_pages, self.v_pages = k_pages, v_pages
-        self.dtype, self.device = k_pages.dtype, k_pages.device
+        self.dtype, self.device, self.index = k_pages.dtype, k_pages.device, k_pages.device.index
         self.desc = PagedCacheDesc(k_pages.device.index, _paged_dtype(k_pages, "k_pages"), k_pages.data_ptr(),
                                    v_pages.data_ptr(), self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
                                    page, head, slot)
@@ -1238,16 +1249,16 @@ class PagedBatch:
 
 
 def _paged_rows(t, name, batch, heads, cache):
-    if t.dim() != 3 or t.shape[0] != batch.n_tokens or t.shape[1] != heads or t.shape[2] != cache.head_dim:
+    if t.shape != (batch.n_tokens, heads, cache.head_dim):
         raise ValueError(f"{name} must be [{batch.n_tokens}, {heads}, {cache.head_dim}]")
-    if t.dtype != cache.dtype or t.device != cache.device:
+    if t.dtype is not cache.dtype or t.get_device() != cache.index:
         raise ValueError(f"{name} must have the cache's dtype and device")
     token, head, unit = t.stride()
-    if unit != 1 and t.shape[2] > 1:
+    if unit != 1 and cache.head_dim > 1:
         raise ValueError(f"the head dimension of {name} must be contiguous")
-    if token == 0 and head == 0 and t.shape[0] * t.shape[1] > 1:
+    if token == 0 and head == 0 and batch.n_tokens * heads > 1:
         raise ValueError(f"{name} must not be one row expanded over tokens and heads")
-    return Rows(t.data_ptr(), token, head)
+    return _pack_rows(t.data_ptr(), token, head)
 
 
 def paged_append_rope(cache: PagedKvCache, batch: PagedBatch, k_new, v_new, rope_theta, q=None, q_out=None):
@@ -1256,53 +1267,53 @@ def paged_append_rope(cache: PagedKvCache, batch: PagedBatch, k_new, v_new, rope
     their positions; queries [n_tokens, n_heads, head_dim], if given, rotated
     into q_out (a new tensor by default; q itself is fine), which is returned.
     rope_theta 0: no rotation (vox_paged_append_rope)."""
+    torch, stream, L = _paged_env()
     ref = batch._for(cache)
     k = _paged_rows(k_new, "k_new", batch, cache.n_kv_heads, cache)
     v = _paged_rows(v_new, "v_new", batch, cache.n_kv_heads, cache)
     heads, qr, qo = 0, None, None
     if q is not None:
-        import torch
-        heads = int(q.shape[1]) if q.dim() == 3 else 0
+        heads = q.shape[1] if q.dim() == 3 else 0
         qr = _paged_rows(q, "q", batch, heads, cache)
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         qo = _paged_rows(q_out, "q_out", batch, heads, cache)
-    _check(lib().vox_paged_append_rope(cache._ref, ref, C.addressof(k), C.addressof(v), rope_theta, heads,
-                                       C.addressof(qr) if qr is not None else None,
-                                       C.addressof(qo) if qo is not None else None, _paged_stream(cache.device)))
+    rc = L.vox_paged_append_rope(cache._ref, ref, k, v, rope_theta, heads, qr, qo, stream(cache.index))
+    if rc:
+        _check(rc)
     return q_out
 
 
-def _paged_attention(cache, batch, prefix, q, sliding_window, n_sinks, scale, out):
-    import torch
+def _paged_attention(cache, batch, prefix, max_prefix, q, sliding_window, n_sinks, scale, out):
+    torch, stream, L = _paged_env()
     ref = batch._for(cache)
-    heads = int(q.shape[1]) if q.dim() == 3 else 0
+    heads = q.shape[1] if q.dim() == 3 else 0
     qr = _paged_rows(q, "q", batch, heads, cache)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     orow = _paged_rows(out, "out", batch, heads, cache)
-    L = lib()
     # the scratch size follows from the host's bounds alone
-    what = (heads, sliding_window, n_sinks, None if prefix is None else prefix.max_len, batch.desc.max_kv_len,
-            cache.dtype, cache.n_kv_heads, cache.head_dim, cache.page_size)
+    what = (heads, sliding_window, n_sinks, max_prefix, batch.desc.max_kv_len, cache.dtype, cache.n_kv_heads,
+            cache.head_dim, cache.page_size)
     n = batch._workspace_bytes.get(what)
     if n is None:
         got = SZ()
         if prefix is None:
             _check(L.vox_paged_attention_workspace(cache._ref, ref, heads, sliding_window, n_sinks, C.byref(got)))
         else:
-            _check(L.vox_paged_prefix_attention_workspace(cache._ref, ref, C.addressof(prefix), heads, sliding_window,
-                                                          n_sinks, C.byref(got)))
+            _check(L.vox_paged_prefix_attention_workspace(cache._ref, ref, prefix, heads, sliding_window, n_sinks,
+                                                          C.byref(got)))
         n = batch._workspace_bytes[what] = got.value
     ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
     wp = ws.data_ptr() if n else None
     if prefix is None:
-        _check(L.vox_paged_attention(cache._ref, ref, C.addressof(qr), heads, sliding_window, n_sinks, scale,
-                                     C.addressof(orow), wp, n, _paged_stream(cache.device)))
+        rc = L.vox_paged_attention(cache._ref, ref, qr, heads, sliding_window, n_sinks, scale, orow, wp, n,
+                                   stream(cache.index))
     else:
-        _check(L.vox_paged_prefix_attention(cache._ref, ref, C.addressof(prefix), C.addressof(qr), heads,
-                                            sliding_window, n_sinks, scale, C.addressof(orow), wp, n,
-                                            _paged_stream(cache.device)))
+        rc = L.vox_paged_prefix_attention(cache._ref, ref, prefix, qr, heads, sliding_window, n_sinks, scale, orow, wp,
+                                          n, stream(cache.index))
+    if rc:
+        _check(rc)
     return out
 
 
@@ -1312,7 +1323,7 @@ def paged_attention(cache: PagedKvCache, batch: PagedBatch, q, sliding_window=0,
     tokens (0: all), its own included, and the first n_sinks of its sequence.
     scale 0 = 1/sqrt(head_dim).  Returns out [n_tokens, n_heads, head_dim];
     rows behind the last sequence are left as they were (vox_paged_attention)."""
-    return _paged_attention(cache, batch, None, q, sliding_window, n_sinks, scale, out)
+    return _paged_attention(cache, batch, None, None, q, sliding_window, n_sinks, scale, out)
 
 
 def paged_prefix_attention(cache: PagedKvCache, batch: PagedBatch, prefix_pages, prefix_len, max_prefix_len, q,
@@ -1322,12 +1333,12 @@ def paged_prefix_attention(cache: PagedKvCache, batch: PagedBatch, prefix_pages,
     max_prefix_len) tokens in the pages prefix_pages (CUDA int32 [pages]).  The
     batch describes the sequences' own tokens behind it; sliding_window and
     n_sinks count from the prefix's first token (vox_paged_prefix_attention)."""
-    import torch
-    if prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or not prefix_pages.is_contiguous() or \
-            prefix_len.dtype != torch.int32 or prefix_len.numel() != 1:
+    torch = _paged_env()[0]
+    if prefix_pages.dtype is not torch.int32 or prefix_pages.dim() != 1 or not prefix_pages.is_contiguous() or \
+            prefix_len.dtype is not torch.int32 or prefix_len.numel() != 1:
         raise ValueError("prefix_pages must be contiguous int32 [pages] and prefix_len int32 [1]")
-    if prefix_pages.device != cache.device or prefix_len.device != cache.device:
+    if prefix_pages.get_device() != cache.index or prefix_len.get_device() != cache.index:
         raise ValueError("the prefix and the cache must be on one device")
-    prefix = PagedPrefixDesc(prefix_pages.data_ptr(), prefix_len.data_ptr(), int(prefix_pages.shape[0]),
-                             int(max_prefix_len))
-    return _paged_attention(cache, batch, prefix, q, sliding_window, n_sinks, scale, out)
+    max_prefix_len = int(max_prefix_len)
+    prefix = _pack_prefix(prefix_pages.data_ptr(), prefix_len.data_ptr(), prefix_pages.shape[0], max_prefix_len)
+    return _paged_attention(cache, batch, prefix, max_prefix_len, q, sliding_window, n_sinks, scale, out)

@@ -9,10 +9,13 @@ namespace {
 
 // ---- append -------------------------------------------------------------------
 //
-// Bound by bytes: every element is read once and written once.  One CTA of 256
-// threads per token: a thread owns one 16-byte column of the head dimension (its
-// pairs' sines and cosines are computed once) and walks over the heads of k, v
-// and q, four rows in flight.
+// Bound by bytes (every element is read once and written once), and for a few
+// tokens by latency.  A thread owns one 16-byte column of a token's rows: its
+// pairs' sines and cosines are computed once, then it walks over the heads of k, v
+// and q with up to 6 rows in flight, loaded before it is known where the token
+// goes.  A CTA of 256 threads takes 4 tokens where there are many (fewer sines,
+// more bytes in flight per CTA: 8.8k tokens 81 -> TBD us), one where there are few
+// (all heads at once).
 //
 // The angle a * theta^(-2c/D) matters modulo a turn only.  turns[c] is the turn
 // fraction per position as a 64-bit binary fraction, so the 64-bit product with
@@ -48,51 +51,82 @@ __device__ __forceinline__ void append_store(T* p, const AppendUnit<T, WIDE>& u)
     }
 }
 
-template <class T, bool WIDE>
+// Where token t goes; one warp calls it.  For up to 32 sequences every lane
+// takes one, so that all their numbers arrive together.
+struct AppendPlace {
+    int seq, p;
+    int64_t first;
+    bool stored_seq;  // part of a sequence with good lengths
+};
+__device__ __forceinline__ AppendPlace append_place(const PagedAppendArgs& a, int t) {
+    AppendPlace r{-1, 0, 0, false};
+    const int lane = threadIdx.x & 31;
+    PagedSeq q{};
+    if (a.n_seqs <= 32) {
+        if (lane < a.n_seqs) {
+            q = paged_seq(a, lane);
+            r.first = a.first_pos ? a.first_pos[lane] : 0;
+        }
+        const unsigned before = __ballot_sync(~0u, lane < a.n_seqs && q.q0 <= t);
+        if (!before) return r;
+        r.seq = 31 - __clz(before);
+        q.q0 = __shfl_sync(~0u, q.q0, r.seq);
+        q.nq = __shfl_sync(~0u, q.nq, r.seq);
+        q.len = __shfl_sync(~0u, q.len, r.seq);
+        q.ok = __shfl_sync(~0u, q.ok, r.seq);
+        r.first = __shfl_sync(~0u, r.first, r.seq);
+    } else {
+        r.seq = paged_seq_of_warp(a, t);
+        if (r.seq < 0) return r;
+        q = paged_seq(a, r.seq);
+        r.first = a.first_pos ? a.first_pos[r.seq] : 0;
+    }
+    if (!q.ok && lane == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+    r.stored_seq = q.ok && t - q.q0 < q.nq;  // else behind the last sequence, or skipped
+    r.p = q.len - q.nq + (t - q.q0);
+    return r;
+}
+
+template <class T, bool WIDE, int TOKENS>
 __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
-    constexpr int N = AppendUnit<T, WIDE>::N, P = N / 2, U = 4;
-    const int chunks = a.hd / N, heads_at_once = 256 / chunks;
-    const int c = threadIdx.x % chunks, h0 = threadIdx.x / chunks;
-    const int t = blockIdx.x;
+    constexpr int N = AppendUnit<T, WIDE>::N, P = N / 2, U = TOKENS > 1 ? 6 : 4, TT = 256 / TOKENS;
+    const int chunks = a.hd / N, heads_at_once = TT / chunks;
+    const int tid = threadIdx.x % TT;
+    const int c = tid % chunks, h0 = tid / chunks;
+    const int t = blockIdx.x * TOKENS + threadIdx.x / TT;
+    if (TOKENS > 1 && t >= a.n_tokens) return;  // whole warps
     const int rows = 2 * a.n_kv + (a.q ? a.n_heads : 0);  // k heads, v heads, q heads
     const bool active = h0 < heads_at_once;
 
-    // where the token goes; the first rows are on their way meanwhile
     AppendUnit<T, WIDE> u[U];
-    auto source = [&](int r) -> const T* {
-        if (r < a.n_kv) return static_cast<const T*>(a.k_new) + t * a.kn_ts + r * a.kn_hs;
-        if (r < 2 * a.n_kv) return static_cast<const T*>(a.v_new) + t * a.vn_ts + (r - a.n_kv) * a.vn_hs;
-        return static_cast<const T*>(a.q) + t * a.q_ts + (r - 2 * a.n_kv) * a.q_hs;
-    };
+    const T* const kn = static_cast<const T*>(a.k_new) + t * a.kn_ts + c * N;
+    const T* const vn = static_cast<const T*>(a.v_new) + t * a.vn_ts + c * N;
+    const T* const qn = static_cast<const T*>(a.q) + t * a.q_ts + c * N;
     auto load = [&](int r0) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int r = r0 + i * heads_at_once;
-            if (active && r < rows) u[i] = append_load<T, WIDE>(source(r) + c * N);
+            if (active && r < rows)
+                u[i] = append_load<T, WIDE>(r < a.n_kv ? kn + r * a.kn_hs
+                                                       : r < 2 * a.n_kv ? vn + (r - a.n_kv) * a.vn_hs : qn + (r - 2 * a.n_kv) * a.q_hs);
         }
     };
     load(h0);
 
-    const int s = paged_seq_of_warp(a, t);
-    if (s < 0) return;
-    const PagedSeq q = paged_seq(a, s);
-    if (!q.ok) {
-        if (threadIdx.x == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
-        return;
-    }
-    if (t - q.q0 >= q.nq) return;  // behind the last sequence
-    const int p = q.len - q.nq + (t - q.q0);
+    const AppendPlace at = append_place(a, t);
+    if (!at.stored_seq) return;
+    const int p = at.p;
     int64_t slot = -1;
     if (p >= 0) {
-        const int page = a.table[s * a.table_stride + (p >> a.page_shift)];
+        const int page = a.table[at.seq * a.table_stride + (p >> a.page_shift)];
         if ((unsigned)page < (unsigned)a.n_pages)
             slot = page * a.page_stride + (p & ((1 << a.page_shift) - 1)) * a.slot_stride;
-        else if (threadIdx.x == 0)
+        else if (tid == 0)
             paged_status(a, VOX_PAGED_BAD_PAGE);
     }
     float sn[P], cs[P];
     if (a.rotate) {
-        const uint64_t pos = (uint64_t)((a.first_pos ? a.first_pos[s] : 0) + p);
+        const uint64_t pos = (uint64_t)(at.first + p);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             if (!active) break;
@@ -101,6 +135,9 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
         }
     }
     if (!active) return;
+    T* const ko = static_cast<T*>(a.k) + slot + c * N;
+    T* const vo = static_cast<T*>(a.v) + slot + c * N;
+    T* const qo = static_cast<T*>(a.q_out) + t * a.qo_ts + c * N;
     for (int r0 = h0; r0 < rows; r0 += U * heads_at_once) {
         if (r0 != h0) load(r0);
 #pragma unroll
@@ -118,14 +155,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
             }
             T* dst;
             if (r >= 2 * a.n_kv)
-                dst = static_cast<T*>(a.q_out) + t * a.qo_ts + (r - 2 * a.n_kv) * a.qo_hs;
+                dst = qo + (r - 2 * a.n_kv) * a.qo_hs;
             else if (slot < 0)
                 continue;
-            else if (is_v)
-                dst = static_cast<T*>(a.v) + slot + (r - a.n_kv) * a.head_stride;
             else
-                dst = static_cast<T*>(a.k) + slot + r * a.head_stride;
-            append_store<T, WIDE>(dst + c * N, u[i]);
+                dst = (is_v ? vo + (r - a.n_kv) * a.head_stride : ko + r * a.head_stride);
+            append_store<T, WIDE>(dst, u[i]);
         }
     }
 }
@@ -339,10 +374,13 @@ cudaError_t by_type(PagedType t, F f) {
 cudaError_t launch_paged_append(PagedType t, const PagedAppendArgs& a, bool wide, cudaStream_t st) {
     return by_type(t, [&](auto x) {
         using T = decltype(x);
-        if (wide)
-            paged_append_kernel<T, true><<<a.n_tokens, 256, 0, st>>>(a);
+        // 4 tokens to a CTA once that still leaves two CTAs to every SM
+        if (wide && a.n_tokens >= 4 * 296)
+            paged_append_kernel<T, true, 4><<<(a.n_tokens + 3) / 4, 256, 0, st>>>(a);
+        else if (wide)
+            paged_append_kernel<T, true, 1><<<a.n_tokens, 256, 0, st>>>(a);
         else
-            paged_append_kernel<T, false><<<a.n_tokens, 256, 0, st>>>(a);
+            paged_append_kernel<T, false, 1><<<a.n_tokens, 256, 0, st>>>(a);
         return cudaGetLastError();
     });
 }
@@ -353,10 +391,9 @@ cudaError_t launch_paged_attn_general(PagedType t, const PagedAttnArgs& a, cudaS
     const size_t smem = general_smem(a.hd);
     return by_type(t, [&](auto x) {
         auto* k = paged_attn_general_kernel<decltype(x)>;
-        if (smem > 48 * 1024) {
-            cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return e;
-        }
+        static PagedKernelSetup setup;
+        cudaError_t e = setup(reinterpret_cast<const void*>(k), (int)general_smem(kPagedMaxHeadDim), false);
+        if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)grid);
         cfg.blockDim = dim3(kGenThreads);

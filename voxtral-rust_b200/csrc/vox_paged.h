@@ -4,6 +4,8 @@
 
 #include <cuda_runtime.h>
 #include <stddef.h>
+
+#include <atomic>
 #include <stdint.h>
 
 namespace vox {
@@ -77,6 +79,26 @@ struct PagedAppendArgs {
     int n_heads, rotate;
     // theta^(-2c/hd) / (2 pi) as a 64-bit binary fraction of a turn
     uint64_t turns[kPagedMaxHeadDim / 2];
+};
+
+// A kernel's limits are raised once per device (a call to the runtime for each
+// launch costs as much as the launch).  One object per kernel.
+class PagedKernelSetup {
+  public:
+    cudaError_t operator()(const void* kernel, int smem_bytes, bool wide_cluster) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = uint64_t(1) << (dev & 63);
+        if (dev < 64 && (done_.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+        if (e == cudaSuccess && wide_cluster) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) done_.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+
+  private:
+    std::atomic<uint64_t> done_{0};
 };
 
 cudaError_t launch_paged_append(PagedType t, const PagedAppendArgs& a, bool wide, cudaStream_t st);

@@ -509,8 +509,8 @@ template <class T, int HD, int NT>
 cudaError_t launch_rows(const PagedAttnArgs& a, int cs, cudaStream_t st) {
     using Cfg = RowsCfg<T, HD, NT>;
     auto* k = paged_attn_rows_kernel<T, HD, NT>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
-    if (e == cudaSuccess && cs > 8) e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static PagedKernelSetup setup;
+    cudaError_t e = setup(reinterpret_cast<const void*>(k), Cfg::SMEM, true);
     if (e != cudaSuccess) return e;
     const int64_t grid = paged_tiles_bound(a, Cfg::ROWS) * a.n_kv * a.splits * cs;
     if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;

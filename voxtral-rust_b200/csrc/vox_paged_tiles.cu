@@ -669,7 +669,8 @@ EncodeFn tensor_map_encoder() {
 template <class T, int HD>
 cudaError_t launch_tiles(const PagedAttnArgs& a, const TileMaps& maps, cudaStream_t st) {
     auto* k = paged_attn_tiles_kernel<T, HD>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TilesCfg<HD>::SMEM);
+    static PagedKernelSetup setup;
+    cudaError_t e = setup(reinterpret_cast<const void*>(k), TilesCfg<HD>::SMEM, false);
     if (e != cudaSuccess) return e;
     const int64_t grid = paged_tiles_bound(a, 2 * kTile) * a.n_kv * a.splits;
     if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
