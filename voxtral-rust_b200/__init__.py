@@ -1276,7 +1276,7 @@ def paged_append_rope(cache: PagedKvCache, batch: PagedBatch, k_new, v_new, rope
         heads = q.shape[1] if q.dim() == 3 else 0
         qr = _paged_rows(q, "q", batch, heads, cache)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qo = _paged_rows(q_out, "q_out", batch, heads, cache)
     rc = L.vox_paged_append_rope(cache._ref, ref, k, v, rope_theta, heads, qr, qo, stream(cache.index))
     if rc:
@@ -1290,7 +1290,7 @@ def _paged_attention(cache, batch, prefix, max_prefix, q, sliding_window, n_sink
     heads = q.shape[1] if q.dim() == 3 else 0
     qr = _paged_rows(q, "q", batch, heads, cache)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     orow = _paged_rows(out, "out", batch, heads, cache)
     # the scratch size follows from the host's bounds alone
     what = (heads, sliding_window, n_sinks, max_prefix, batch.desc.max_kv_len, cache.dtype, cache.n_kv_heads,

@@ -387,8 +387,8 @@ extern "C" int vox_paged_append_rope(const vox_paged_cache* c, const vox_paged_b
         // theta^(-2c/D) / (2 pi) in units of 2^-64 turn, by repeated products in
         // 64-bit-mantissa arithmetic
         const long double ratio = powl((long double)theta, -2.0L / (long double)c->head_dim);
-        long double f = 0.15915494309189533576888376337251436L;
-        for (size_t i = 0; i < c->head_dim / 2; ++i, f *= ratio) a.turns[i] = (uint64_t)ldexpl(f, 64);
+        long double f = 0.15915494309189533576888376337251436L * 18446744073709551616.0L;
+        for (size_t i = 0; i < c->head_dim / 2; ++i, f *= ratio) a.turns[i] = (uint64_t)f;
     }
     // 16-byte columns where every row starts on a 16-byte boundary
     const bool wide = c->head_dim * type_size(k.type) % 16 == 0 &&
