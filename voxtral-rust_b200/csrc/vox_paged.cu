@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     float* q_s = sm;                    // [R][hd]
     float* k_s = q_s + R * hd;          // [32][hd + 1]
     float* v_s = k_s + kGenKeys * (hd + 1);  // [32][hd]
-    __shared__ PagedTileRows<R> rows;
+    __shared__ int tok_s[R], head_s[R], p_row_s[R];
     __shared__ float p_s[R][kGenKeys], alpha_s[R], l_s[R], m_s[R];
     __shared__ int64_t off_s[kGenKeys];
 
@@ -194,15 +194,18 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     const int tile = blockIdx.x / a.splits / a.n_kv;
     PagedKeys ks;
     pdl_allow_dependents();
-    if (!paged_tile_rows(a, tile, rows, &ks)) {
+    PagedTileRows rows;
+    if (!paged_tile_rows<R>(a, tile, rows, &ks)) {
         pdl_wait_prior_grids();
         return;
     }
+    if (tid < R) tok_s[tid] = rows.tok, head_s[tid] = h * a.group + rows.g, p_row_s[tid] = rows.p;
+    __syncthreads();
     for (int i = tid; i < R * hd; i += kGenThreads) {
         const int r = i / hd, d = i % hd;
         float x = 0.f;
-        if (rows.tok[r] >= 0)
-            x = to_f32(static_cast<const T*>(a.q)[rows.tok[r] * a.q_ts + (h * a.group + rows.g[r]) * a.q_hs + d]);
+        if (tok_s[r] >= 0)
+            x = to_f32(static_cast<const T*>(a.q)[tok_s[r] * a.q_ts + head_s[r] * a.q_hs + d]);
         q_s[i] = x;
     }
     const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 5);
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
             const int r = warp + 4 * i;
             float s = 0.f;
             for (int d = 0; d < hd; ++d) s = fmaf(q_s[r * hd + d], k_s[lane * (hd + 1) + d], s);
-            const bool seen = rows.tok[r] >= 0 && paged_sees(rows.p[r], j0 + lane, ks.len, a.window, ks.sinks);
+            const bool seen = tok_s[r] >= 0 && paged_sees(p_row_s[r], j0 + lane, ks.len, a.window, ks.sinks);
             s = seen ? s * a.scale_log2 : kNegInf;
             float top = s;
             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
@@ -265,9 +268,9 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
     }
     __syncthreads();
     for (int r = 0; r < R; ++r) {
-        const int tok = rows.tok[r];
+        const int tok = tok_s[r];
         if (tok < 0) continue;
-        const int head = h * a.group + rows.g[r];
+        const int head = head_s[r];
         const float ls = l_s[r];
         const int64_t at = ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head;
         if (a.part_o && tid == 0) a.part_ml[at] = make_float2(m_s[r], ls);

@@ -182,76 +182,57 @@ __device__ __noinline__ void paged_redo_row(const PagedAttnArgs& a, PagedKeys ks
         }
 }
 
-// A tile's query rows: token (-1: no such row), index in the keys' numbering,
-// head within the kv head's group.
-template <int ROWS>
+// A tile's query rows, up to 32: lane r of every warp has row r's token (-1: no
+// such row), index in the keys' numbering and head within the kv head's group;
+// pmin and pmax are the smallest and largest index.  Every warp finds them for
+// itself, so that its first keys are asked for before any block-wide barrier.
 struct PagedTileRows {
-    int tok[ROWS], p[ROWS], g[ROWS];
-    int seq, place, pmin, pmax;
+    int tok, p, g, pmin, pmax;
 };
-
-// Fills the rows of tile `tile` (in shared memory) and what they attend to.
-// All threads of the block call it (at least ROWS and at least a warp);
-// false, for the whole block alike: the tile has no rows.
 template <int ROWS>
-__device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile, PagedTileRows<ROWS>& rows,
-                                                PagedKeys* ks) {
-    const int tid = threadIdx.x;
+__device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile, PagedTileRows& rows, PagedKeys* ks) {
+    const int lane = threadIdx.x & 31;
     const int plen = a.pfx_len ? paged_prefix_len(a) : 0;
     if (plen < 0) {
-        if (tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        if (threadIdx.x == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
         return false;
     }
-    if (tid == 0) rows.pmin = 0x7FFFFFFF, rows.pmax = -0x7FFFFFFF;
-    int tok = -1, p = -1;
+    rows.tok = rows.p = -1;
     int64_t row;
     if (!a.in_prefix) {
-        if (tid < 32) {
-            int place;
-            const int s = paged_find_tile(a, tile, ROWS, &place);
-            if (tid == 0) rows.seq = s, rows.place = place;
-        }
-        __syncthreads();
-        const int s = rows.seq;
+        int place;
+        const int s = paged_find_tile(a, tile, ROWS, &place);
         if (s < 0) return false;
         const PagedSeq q = paged_seq(a, s);
-        if (!q.ok && tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        if (!q.ok && threadIdx.x == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
         if (q.nq == 0) return false;
-        row = (int64_t)rows.place * ROWS + tid;
-        if (tid < ROWS && row < (int64_t)q.nq * a.group) {
+        row = (int64_t)place * ROWS + lane;
+        if (lane < ROWS && row < (int64_t)q.nq * a.group) {
             const int i = (int)(row / a.group);
-            tok = q.q0 + i;
-            p = q.len - q.nq + i;
+            rows.tok = q.q0 + i;
+            rows.p = q.len - q.nq + i;
         }
         ks->table = a.table + s * a.table_stride;
         ks->len = q.len;
         ks->sinks = max(0, a.sinks - plen);
     } else {
-        __syncthreads();
-        row = (int64_t)tile * ROWS + tid;
-        if (tid < ROWS && row < (int64_t)a.n_tokens * a.group) {
+        row = (int64_t)tile * ROWS + lane;
+        if (lane < ROWS && row < (int64_t)a.n_tokens * a.group) {
             const int t = (int)(row / a.group);
             const int s = paged_seq_of(a, t);
             if (s >= 0) {
                 const PagedSeq q = paged_seq(a, s);
                 if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);
-                if (t - q.q0 < q.nq) tok = t, p = plen + q.len - q.nq + (t - q.q0);
+                if (t - q.q0 < q.nq) rows.tok = t, rows.p = plen + q.len - q.nq + (t - q.q0);
             }
         }
         ks->table = a.pfx_pages;
         ks->len = plen;
         ks->sinks = a.sinks;
     }
-    if (tid < ROWS) {
-        rows.tok[tid] = tok;
-        rows.p[tid] = p;
-        rows.g[tid] = (int)(row % a.group);
-        if (tok >= 0) {
-            atomicMin(&rows.pmin, p);
-            atomicMax(&rows.pmax, p);
-        }
-    }
-    __syncthreads();
+    rows.g = (int)(row % a.group);
+    rows.pmin = __reduce_min_sync(~0u, rows.tok >= 0 ? rows.p : 0x7FFFFFFF);
+    rows.pmax = __reduce_max_sync(~0u, rows.tok >= 0 ? rows.p : -0x7FFFFFFF);
     return rows.pmin <= rows.pmax;
 }
 

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     constexpr int ROWS = Cfg::ROWS, U = Cfg::UNITS, UNIT = Cfg::UNIT, C = Cfg::CHUNKS, OS = Cfg::OS;
     constexpr int kWarps = Cfg::WARPS, kThreads = 32 * kWarps;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ PagedTileRows<ROWS> rows;
+    __shared__ int tok_s[ROWS], head_s[ROWS], p_s[ROWS];
     __shared__ float m_s[kWarps][ROWS], l_s[kWarps][ROWS], cm_s[ROWS], cl_s[ROWS];
     __shared__ float wc_s[16][ROWS], tot_s[ROWS];
     __shared__ int odd_s[ROWS];
@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     const int tile = (int)(gridDim.x / cs / a.splits / a.n_kv) - 1 - unit / a.splits / a.n_kv;
     PagedKeys ks;
     pdl_allow_dependents();
-    if (!paged_tile_rows(a, tile, rows, &ks)) {  // the whole cluster alike
+    PagedTileRows rows;
+    if (!paged_tile_rows<ROWS>(a, tile, rows, &ks)) {  // the whole cluster alike
         pdl_wait_prior_grids();
         return;
     }
@@ -225,9 +226,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         for (int i = tid; i < ROWS * C; i += kThreads) {
             const int r = i / C, c = i % C;
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (rows.tok[r] >= 0)
-                v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + rows.tok[r] * a.q_ts +
-                                                    (h * a.group + rows.g[r]) * a.q_hs + c * E);
+            const int tok = __shfl_sync(~0u, rows.tok, r), head = h * a.group + __shfl_sync(~0u, rows.g, r);
+            if (tok >= 0) v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.q_ts + head * a.q_hs + c * E);
             const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) p[n][e] = rows.p[n * 8 + 2 * t + e];
+        for (int e = 0; e < 2; ++e) p[n][e] = __shfl_sync(~0u, rows.p, n * 8 + 2 * t + e);
+    if (tid < ROWS) tok_s[tid] = rows.tok, head_s[tid] = h * a.group + rows.g, p_s[tid] = rows.p;
 
     __syncthreads();
 
@@ -446,9 +447,9 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     // A value that is not finite may have come from a key that a row does not
     // see (0 x inf): such rows are done again key by key.
     for (int r = warp; r < ROWS; r += kWarps) {
-        if (!odd_s[r] || rows.tok[r] < 0) continue;
+        if (!odd_s[r] || tok_s[r] < 0) continue;
         float acc[HD / 32];
-        paged_redo_row<T, HD / 32>(a, ks, kb, kKeys, b0, b1, h, rows.tok[r], h * a.group + rows.g[r], rows.p[r], cm_s[r], acc);
+        paged_redo_row<T, HD / 32>(a, ks, kb, kKeys, b0, b1, h, tok_s[r], head_s[r], p_s[r], cm_s[r], acc);
 #pragma unroll
         for (int e = 0; e < HD / 32; ++e) body[r * OS + lane + 32 * e] = acc[e];
     }
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     __syncthreads();
     const int i0 = ROWS * V4 * rank / cs, i1 = ROWS * V4 * (rank + 1) / cs;
     for (int i = i0 + tid; i < i1; i += kThreads) {
-        const int r = i / V4, d = (i % V4) * 4, tok = rows.tok[r];
+        const int r = i / V4, d = (i % V4) * 4, tok = tok_s[r];
         if (tok < 0) continue;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(body + r * OS + d, c));
             v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
         }
-        const int head = h * a.group + rows.g[r];
+        const int head = head_s[r];
         const float total = tot_s[r];
         if (a.part_o) {
             const int64_t at = ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head;
