@@ -298,6 +298,45 @@ def test_prefix_window_and_sinks(V, dtype, window, sinks):
     assert int(c.status) == 0
 
 
+# Long enough, or with enough rows, to be computed once for all sequences (a short
+# prefix is the first part of every sequence's keys).
+SHARED = [
+    # heads, kv, dim, prefix, q_len, kv_len
+    (8, 2, 64, 2100, (1,) * 40, tuple(range(1, 41))),
+    (8, 2, 128, 1111, (1, 0, 2, 1) * 10, (30, 4, 9, 1) * 10),
+    (8, 1, 128, 130, (5, 1, 4), (40, 1, 3)),       # 40 rows a sequence: tcgen05 for its own keys too
+    (4, 4, 128, 3000, (1,) * 12, (7,) * 12),       # 12 rows for the prefix
+    (12, 2, 80, 1200, (1, 2) * 30, (3, 20) * 30),  # CUDA cores
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim,prefix,q_len,kv_len", SHARED)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3), (900, 1000)])
+def test_shared_prefix(V, dtype, heads, kv, dim, prefix, q_len, kv_len, window, sinks):
+    c = Case(V, torch, dtype, heads, kv, dim, 16, q_len, kv_len, window, sinks, prefix=prefix, seed=23, spare_tokens=3)
+    out = torch.full_like(c.q, 3.0)
+    c.run(out=out)
+    assert bool((out[sum(q_len):] == 3.0).all())
+    c.check(out)
+    assert int(c.status) == 0
+
+
+def test_bad_shared_prefix_is_reported(V):
+    c = Case(V, torch, "bf16", 8, 2, 128, 16, (1,) * 40, (5,) * 40, prefix=1200, seed=24)
+    want = c.run()
+    for n in (-1, 1201):
+        c.pre_len.fill_(n)
+        c.status.zero_()
+        out = torch.full_like(want, 4.0)
+        c.run(out=out)
+        assert int(c.status) == V.PAGED_BAD_LENGTH and bool((out == 4.0).all())
+    c.pre_len.fill_(1200)
+    c.status.zero_()
+    c.pre_dev[7] = 1 << 30
+    assert bool(torch.isfinite(c.run()).all()) and int(c.status) == V.PAGED_BAD_PAGE
+
+
 def test_prefix_equals_attention_on_whole_sequences(V):
     """The same tokens as one paged sequence each: equal up to the rounding of
     weights and results (two of each)."""
@@ -364,7 +403,7 @@ def test_graph_replays_follow_the_device_arrays(V):
 
 def test_two_graphs_and_two_streams_do_not_share_scratch(V):
     cases = [Case(V, torch, "bf16", 8, 2, 128, 16, (1,), (900 + 40 * i,), seed=18 + i) for i in range(2)]
-    cases += [Case(V, torch, "bf16", 8, 2, 128, 16, (1,) * 9, (9,) * 9, prefix=700 + i, seed=28 + i) for i in range(2)]
+    cases += [Case(V, torch, "bf16", 8, 2, 128, 16, (1,) * 9, (9,) * 9, prefix=3700 + i, seed=28 + i) for i in range(2)]
     want = [c.run() for c in cases]
     graphs, outs = [], []
     for c in cases:
@@ -393,7 +432,8 @@ def test_two_graphs_and_two_streams_do_not_share_scratch(V):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_results_do_not_depend_on_the_run(V, dtype):
-    for q_len, kv_len, prefix in (((1, 1), (3000, 17), 0), ((200,), (1300,), 0), ((1,) * 20, (30,) * 20, 1000)):
+    for q_len, kv_len, prefix in (((1, 1), (3000, 17), 0), ((200,), (1300,), 0), ((1,) * 20, (30,) * 20, 1000),
+                                 ((1,) * 40, (30,) * 40, 2000)):
         c = Case(V, torch, dtype, 8, 2, 128, 16, q_len, kv_len, prefix=prefix, seed=19, poison=False)
         first = c.run()
         for _ in range(5):
@@ -465,9 +505,9 @@ def test_empty_batches(V):
 
 
 def test_workspace_is_checked(V):
-    c = Case(V, torch, "bf16", 8, 2, 64, 16, (1, 1), (5, 9), prefix=40, seed=22, max_kv=16)
+    c = Case(V, torch, "bf16", 8, 2, 64, 16, (1,) * 60, (5, 9) * 30, prefix=1100, seed=22, max_kv=16)
     L = V.lib()
-    pre = V.PagedPrefixDesc(c.pre_dev.data_ptr(), c.pre_len.data_ptr(), len(c.pre), 40)
+    pre = V.PagedPrefixDesc(c.pre_dev.data_ptr(), c.pre_len.data_ptr(), len(c.pre), 1100)
     n = C.c_size_t()
     assert L.vox_paged_prefix_attention_workspace(c.cache._ref, c.batch._ref, C.byref(pre), 8, 0, 0, C.byref(n)) == 0
     assert n.value > 0

@@ -215,7 +215,7 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     // equal shares; more, where the bytes bound the call (one decode step's rows),
     // into about four waves, which evens out ragged lengths: 96 sequences of up
     // to 8192 visible keys 411 us against 434 with half as many CTAs.
-    const int64_t slots = 148 * (t != PagedType::F32 || p.nt == 1 ? 2 : 1);
+    const int64_t slots = 148 * 2;
     const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (4 * slots + units - 1) / units : 1;
     // At least 64 keys to a CTA of a cluster (one stream of 1536 tokens: 15 us
     // through clusters alone, 20 us with a merge behind them), 512 where there
@@ -231,6 +231,7 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
 // What a call launches.
 struct AttnPlan {
     KeysPlan own, prefix;
+    bool joined = false;   // the prefix as the first part of every sequence's keys
     int parts = 1;         // partial results of a row
     bool partial = false;  // through the workspace
     size_t ml_bytes = 0, bytes = 0;
@@ -239,7 +240,7 @@ struct AttnPlan {
 AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_batch* b, const vox_paged_prefix* p,
                         size_t n_heads, size_t window, size_t sinks) {
     AttnPlan plan;
-    const int64_t group = (int64_t)(n_heads / c->n_kv_heads);
+    const int64_t group = (int64_t)(n_heads / c->n_kv_heads), all_rows = (int64_t)(b->n_tokens * n_heads);
     auto visible = [&](size_t len) {
         return (int64_t)(window ? std::min(len, window + b->max_q_len + std::min(sinks, len)) : len);
     };
@@ -248,12 +249,17 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
     a.n_seqs = (int)b->n_seqs;
     a.max_q = (int)b->max_q_len;
     a.group = (int)group;
-    const int64_t all_rows = (int64_t)(b->n_tokens * n_heads);
-    plan.own = plan_keys(c, t, (int64_t)b->max_q_len * group, all_rows, visible(b->max_kv_len),
+    const int64_t rows = (int64_t)b->max_q_len * group;
+    // A short prefix is read again for every sequence, out of the L2, as the first
+    // part of its keys: one launch where the shared form takes three (8 hypotheses
+    // behind 639 tokens: 10 us against 17).  32 MB are about 4 us of it.
+    plan.joined = p && rows <= 32 &&
+                  (double)b->n_seqs * (double)p->max_len * (double)(c->n_kv_heads * c->head_dim * 2 * type_size(t)) <= 32e6;
+    plan.own = plan_keys(c, t, rows, all_rows, visible(b->max_kv_len + (plan.joined ? p->max_len : 0)),
                          [&](int n) { return paged_tiles_bound(a, n); });
     plan.parts = plan.own.splits;
-    if (p) {
-        a.in_prefix = 1;
+    if (p && !plan.joined) {
+        a.keys_of = PagedKeysOf::PREFIX;
         plan.prefix = plan_keys(c, t, (int64_t)b->n_tokens * group, all_rows, visible(p->max_len),
                                 [&](int n) { return paged_tiles_bound(a, n); });
         plan.parts += plan.prefix.splits;
@@ -339,16 +345,17 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
     const bool aligned = aligned16(a.k, k.type, {a.page_stride, a.head_stride, a.slot_stride}) &&
                          aligned16(a.v, k.type, {}) && aligned16(a.q, k.type, {a.q_ts, a.q_hs}) &&
                          aligned16(a.out, k.type, {a.o_ts, a.o_hs});
-    // The prefix after the sequences' own keys: its launch starts while the other
-    // drains, and waits for it only at its end.
-    a.part0 = plan.prefix.splits * (p != nullptr);
+    const bool shared = p && !plan.joined;
+    a.keys_of = plan.joined ? PagedKeysOf::JOINED : PagedKeysOf::OWN;
+    a.part0 = shared ? plan.prefix.splits : 0;
     TRY(launched(launch_keys(k.type, a, plan.own, aligned, st), "paged attention"));
-    if (p) {
-        PagedAttnArgs shared = a;
-        shared.in_prefix = 1;
-        shared.part0 = 0;
-        shared.follows = 1;
-        TRY(launched(launch_keys(k.type, shared, plan.prefix, aligned, st), "prefix attention"));
+    if (shared) {
+        // its launch starts while the other drains, and waits for it only at its end
+        PagedAttnArgs s = a;
+        s.keys_of = PagedKeysOf::PREFIX;
+        s.part0 = 0;
+        s.follows = 1;
+        TRY(launched(launch_keys(k.type, s, plan.prefix, aligned, st), "prefix attention"));
     }
     if (plan.partial) TRY(launched(launch_paged_merge(k.type, a, plan.parts, st), "paged merge"));
     return VOX_OK;

@@ -135,20 +135,27 @@ __device__ __forceinline__ bool paged_sees(int p, int j, int len, int window, in
     return j <= p && j < len && (window == 0 || j < sinks || j > p - window);
 }
 
-// What a tile of rows attends to: its table row, length and sink count.
+// What a tile of rows attends to: keys 0..len-1, of which the first plen are in
+// the pages pfx and the others in the pages of a table row; and the sink count.
 struct PagedKeys {
     const int32_t* table;
     int len, sinks;
+    const int32_t* pfx;
+    int plen;
+    __device__ __forceinline__ int page(int j, int shift) const {
+        return j < plen ? pfx[j >> shift] : table[(j - plen) >> shift];
+    }
+    __device__ __forceinline__ int slot(int j, int shift) const { return (j < plen ? j : j - plen) & ((1 << shift) - 1); }
 };
 
 // Offset of key j's row of kv head h, or -1 where its page id is bad.
 __device__ __forceinline__ int64_t paged_row(const PagedAttnArgs& a, const PagedKeys& ks, int j, int h) {
-    const int page = ks.table[j >> a.page_shift];
+    const int page = ks.page(j, a.page_shift);
     if ((unsigned)page >= (unsigned)a.n_pages) {
         paged_status(a, VOX_PAGED_BAD_PAGE);
         return -1;
     }
-    return page * a.page_stride + h * a.head_stride + (j & ((1 << a.page_shift) - 1)) * a.slot_stride;
+    return page * a.page_stride + h * a.head_stride + ks.slot(j, a.page_shift) * a.slot_stride;
 }
 
 // One row again, key by key: acc[e] = sum of 2^(score - m) v[lane + 32 e] over
@@ -199,7 +206,9 @@ __device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile
     }
     rows.tok = rows.p = -1;
     int64_t row;
-    if (!a.in_prefix) {
+    ks->pfx = nullptr;
+    ks->plen = 0;
+    if (a.keys_of != PagedKeysOf::PREFIX) {
         int place;
         const int s = paged_find_tile(a, tile, ROWS, &place);
         if (s < 0) return false;
@@ -213,8 +222,16 @@ __device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile
             rows.p = q.len - q.nq + i;
         }
         ks->table = a.table + s * a.table_stride;
-        ks->len = q.len;
-        ks->sinks = max(0, a.sinks - plen);
+        if (a.keys_of == PagedKeysOf::JOINED) {
+            ks->pfx = a.pfx_pages;
+            ks->plen = plen;
+            ks->len = plen + q.len;
+            ks->sinks = a.sinks;
+            if (rows.tok >= 0) rows.p += plen;
+        } else {
+            ks->len = q.len;
+            ks->sinks = max(0, a.sinks - plen);
+        }
     } else {
         row = (int64_t)tile * ROWS + lane;
         if (lane < ROWS && row < (int64_t)a.n_tokens * a.group) {

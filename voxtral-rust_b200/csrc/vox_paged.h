@@ -14,6 +14,8 @@ enum class PagedType : int { F32, F16, BF16 };
 
 constexpr int kPagedMaxHeadDim = 256;
 
+enum class PagedKeysOf : int { OWN, PREFIX, JOINED };
+
 // Arguments of every paged attention kernel.  Counts and token indices are
 // 32 bits (the host checks them); every offset into a tensor is 64 bits.
 struct PagedAttnArgs {
@@ -29,11 +31,13 @@ struct PagedAttnArgs {
     const int32_t* kv_len;
     const int32_t* table;
     uint32_t* status;
-    // shared prefix (pfx_len null: none).  in_prefix 1: the keys are the
-    // prefix's and the rows all tokens of the batch; 0: each sequence's own.
+    // shared prefix (pfx_len null: none), and which keys a launch attends to:
+    // each sequence's own, the prefix's (the rows are then all tokens of the
+    // batch), or for each sequence the prefix's and then its own.
     const int32_t* pfx_pages;
     const int32_t* pfx_len;
-    int pfx_n_pages, pfx_max, in_prefix;
+    int pfx_n_pages, pfx_max;
+    PagedKeysOf keys_of;
     // queries and outputs
     const void* q;
     int64_t q_ts, q_hs;
@@ -56,7 +60,7 @@ struct PagedAttnArgs {
 
 // Upper bound on the tiles of `rows` query rows, from the host's bounds alone.
 inline int64_t paged_tiles_bound(const PagedAttnArgs& a, int rows) {
-    if (a.in_prefix) return ((int64_t)a.n_tokens * a.group + rows - 1) / rows;
+    if (a.keys_of == PagedKeysOf::PREFIX) return ((int64_t)a.n_tokens * a.group + rows - 1) / rows;
     if ((int64_t)a.max_q * a.group <= rows) return a.n_seqs;
     return (int64_t)a.n_tokens * a.group / rows + a.n_seqs;
 }

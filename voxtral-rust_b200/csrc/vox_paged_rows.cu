@@ -46,8 +46,8 @@ struct RowsCfg {
     static constexpr int ROW_BYTES = HD * (int)sizeof(T);
     static constexpr int CHUNKS = ROW_BYTES / 16;
     static constexpr int UNIT = kKeys * ROW_BYTES;
-    static constexpr int WARPS = F32 && (NT == 4 || (NT == 2 && HD == 128)) ? 8 : 4;
-    static constexpr int UNITS = F32 ? (HD == 128 ? (NT == 4 ? 2 : 3) : (NT == 4 ? 4 : 6)) : (HD == 128 ? 6 : 8);
+    static constexpr int WARPS = 4;
+    static constexpr int UNITS = F32 ? (HD == 128 ? (NT == 1 ? 3 : 2) : (NT == 4 ? 4 : 6)) : (HD == 128 ? 6 : 8);
     static constexpr int RING = WARPS * UNITS * UNIT;
     static constexpr int OS = HD + 4;  // row stride of the partial results
     static constexpr int QF = F32 ? HD / 8 * NT * 512 : HD / 32 * NT * 512;
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     auto page_of = [&](int i) {
         if (i >= b1 || lane >= kKeys) return -2;
         const int j = kb.block(i) * kKeys + lane;
-        return kb.seen(j) ? ks.table[j >> a.page_shift] : -2;
+        return kb.seen(j) ? ks.page(j, a.page_shift) : -2;
     };
     // where this lane's key of block i begins; -1: zeros
     auto offset_of = [&](int i, int page) -> int64_t {
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             return -1;
         }
         const int j = kb.block(i) * kKeys + lane;
-        return page * a.page_stride + (j & ((1 << a.page_shift) - 1)) * a.slot_stride;
+        return page * a.page_stride + ks.slot(j, a.page_shift) * a.slot_stride;
     };
     auto issue = [&](const T* base, int64_t off, int slot, bool is_v) {
         const uint32_t dst = ring + slot * UNIT;

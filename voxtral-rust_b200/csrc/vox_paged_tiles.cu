@@ -280,14 +280,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     // every warp looks for itself: one block-wide barrier in the whole prologue
     int place = tile, seq = 0;
-    if (!a.in_prefix) seq = paged_find_tile(a, tile, 2 * kTile, &place);
+    if (a.keys_of == PagedKeysOf::OWN) seq = paged_find_tile(a, tile, 2 * kTile, &place);
     if (seq < 0) {
         pdl_wait_prior_grids();
         return;
     }
-    PagedKeys ks{a.pfx_pages, plen, a.sinks};
+    PagedKeys ks{a.pfx_pages, plen, a.sinks, nullptr, 0};
     int tok = -1, p = -1, head = 0;
-    if (!a.in_prefix) {
+    if (a.keys_of == PagedKeysOf::OWN) {
         const PagedSeq q = paged_seq(a, seq);
         if (!q.ok && tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
         ks.table = a.table + seq * a.table_stride;
