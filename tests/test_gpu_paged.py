@@ -138,6 +138,52 @@ def test_append_reports_bad_pages_and_lengths(V):
 
 # ---- attention ---------------------------------------------------------------
 
+# Batches whose host bounds ask for equal shares of all keys (48 MB and more)
+LONG = [
+    # dtype, heads, kv, dim, q_len, kv_len, window, sinks
+    ("f32", 32, 8, 128, (1,) * 8, (1036, 17, 3000, 0, 1, 900, 16, 257), 0, 0),
+    ("bf16", 8, 8, 128, (1, 0, 2, 1, 1) * 3, (1, 5, 2000, 333, 48) * 3, 700, 5),
+    ("f16", 16, 8, 64, (2, 1, 8) * 20, (900, 64, 8) * 20, 0, 0),
+    ("bf16", 8, 8, 128, (1,) * 100, (1, 2, 3, 4) * 24 + (800, 1, 1, 0), 0, 0),   # fewer blocks than shares
+    ("bf16", 16, 8, 128, (1,) * 3, (5000, 16, 1), 4500, 40),
+]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,q_len,kv_len,window,sinks", LONG)
+@pytest.mark.parametrize("prefix", [0, 30])
+def test_decode_in_equal_shares(V, dtype, heads, kv, dim, q_len, kv_len, window, sinks, prefix):
+    c = Case(V, torch, dtype, heads, kv, dim, 16, q_len, kv_len, window, sinks, prefix=prefix, seed=25, spare_tokens=2)
+    out = torch.full_like(c.q, 3.0)
+    c.run(out=out)
+    assert bool((out[sum(q_len):] == 3.0).all())
+    c.check(out)
+    assert int(c.status) == 0
+    again = torch.full_like(c.q, 3.0)
+    c.run(out=again)
+    assert torch.equal(out, again)
+
+
+def test_bad_sequences_in_equal_shares(V):
+    c = Case(V, torch, "bf16", 8, 8, 128, 16, (1,) * 8, (900, 1600, 30, 700, 1, 1500, 44, 90), seed=26, poison=False)
+    want = c.run()
+    c.kv[1] = 1601
+    c.kv[4] = -1
+    c.table_dev[5, 3] = -2
+    out = torch.full_like(want, 9.0)
+    c.run(out=out)
+    assert int(c.status) == V.PAGED_BAD_LENGTH | V.PAGED_BAD_PAGE
+    for s in range(8):
+        if s in (1, 4):
+            assert bool((out[s] == 9.0).all())
+        elif s != 5:
+            # shares begin elsewhere: the same terms in another order
+            assert float((out[s] - want[s]).abs().max()) <= 2.0 ** -6 * float(want[s].abs().max())
+    c.q_start.fill_(0)  # no tokens at all
+    out.fill_(9.0)
+    c.run(out=out)
+    assert bool((out == 9.0).all())
+
+
 SHAPES = [  # heads, kv_heads, dim
     (32, 8, 128), (8, 1, 64), (4, 4, 128), (10, 2, 64), (7, 1, 128), (6, 2, 80), (2, 1, 256), (3, 3, 6),
 ]

@@ -25,6 +25,8 @@
 // joins.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "vox_paged.cuh"
 
 namespace cg = cooperative_groups;
@@ -130,7 +132,87 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
-template <class T, int HD, int NT>
+// ---- equal shares --------------------------------------------------------------
+//
+// Where sequences of different lengths (at most one tile each) are read from HBM,
+// a CTA takes an equal share of all (sequence, kv head) units' 16-key blocks in
+// one line, instead of a cluster taking a unit: 8 f32 streams of 1036..3513 tokens
+// 43 us with 4 CTAs a unit, 33 us in equal shares.  A share's first piece may end
+// a unit that began in the share before, its last one may begin a unit that goes
+// on: those two are written to the share's slots, and a second launch joins each
+// unit in the share that it begins in.
+
+constexpr int kShareSeqs = kPagedShareSeqs;  // sequences whose running block counts fit
+
+struct ShareSums {
+    int64_t all;               // blocks of all units
+    int sums[kShareSeqs + 1];  // blocks of one kv head of the sequences before
+};
+
+// The block cost of a sequence: at least 1, so that a token that sees nothing is
+// written too; 0 without tokens.
+__device__ __forceinline__ int share_cost(const PagedAttnArgs& a, int s, int plen) {
+    const PagedSeq q = paged_seq(a, s);
+    if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);
+    if (q.nq == 0) return 0;
+    const int len = plen + q.len;
+    return max(1, paged_key_blocks(len - q.nq, len - 1, len, a.window, a.sinks, 4).total);
+}
+
+// All threads of the block call it; false: nothing to do.
+__device__ __forceinline__ bool share_sums(const PagedAttnArgs& a, ShareSums& sh) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int plen = a.pfx_len ? paged_prefix_len(a) : 0;
+    if (plen < 0) {
+        if (tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
+        return false;
+    }
+    for (int s = tid; s < a.n_seqs; s += blockDim.x) sh.sums[s + 1] = share_cost(a, s, plen);
+    __syncthreads();
+    if (tid < 32) {
+        int before = 0;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            int n = s0 + lane < a.n_seqs ? sh.sums[s0 + lane + 1] : 0;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(~0u, n, o);
+                if (lane >= o) n += up;
+            }
+            if (s0 + lane < a.n_seqs) sh.sums[s0 + lane + 1] = before + n;
+            before += __shfl_sync(~0u, n, 31);
+        }
+        if (lane == 0) sh.sums[0] = 0, sh.all = (int64_t)before * a.n_kv;
+    }
+    __syncthreads();
+    return sh.all > 0;
+}
+
+// The unit that holds block x of the line, and where in it.
+struct ShareUnit {
+    int seq, head, block, cost;
+    int64_t start;
+};
+__device__ __forceinline__ ShareUnit share_unit(const PagedAttnArgs& a, const ShareSums& sh, int64_t x) {
+    const int want = (int)(x / a.n_kv);
+    int lo = 0, hi = a.n_seqs;  // the last s with sums[s] <= want has a cost above 0
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sh.sums[mid] <= want) lo = mid; else hi = mid;
+    }
+    ShareUnit u;
+    u.seq = lo;
+    u.cost = sh.sums[lo + 1] - sh.sums[lo];
+    const int64_t r = x - (int64_t)sh.sums[lo] * a.n_kv;
+    u.head = (int)(r / u.cost);
+    u.block = (int)(r - (int64_t)u.head * u.cost);
+    u.start = x - u.block;
+    return u;
+}
+__device__ __forceinline__ int64_t share_begin(const ShareSums& sh, int c, int n) { return sh.all * c / n; }
+
+// The rows' results in a share's slots: [share][slot][row] (m, l) and [.. row][HD].
+__device__ __forceinline__ int64_t share_slot(int share, int slot, int rows) { return ((int64_t)share * 2 + slot) * rows; }
+
+template <class T, int HD, int NT, bool SHARES>
 __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD, NT>::PER_SM)
     paged_attn_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     using Cfg = RowsCfg<T, HD, NT>;
@@ -146,14 +228,32 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     uint4* qf = reinterpret_cast<uint4*>(smem + Cfg::BODY);
 
     const cg::cluster_group cluster = cg::this_cluster();
-    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int cs = SHARES ? 1 : (int)cluster.num_blocks(), rank = SHARES ? 0 : (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int unit = blockIdx.x / cs;
-    const int z = unit % a.splits, h = (unit / a.splits) % a.n_kv;
-    // last tiles first: a sequence's later tokens see more keys
-    const int tile = (int)(gridDim.x / cs / a.splits / a.n_kv) - 1 - unit / a.splits / a.n_kv;
-    PagedKeys ks;
     pdl_allow_dependents();
+    __shared__ std::conditional_t<SHARES, ShareSums, char> share;
+    int64_t x = 0, x_end = 0;
+    if constexpr (SHARES) {
+        if (!share_sums(a, share)) return;
+        x = share_begin(share, blockIdx.x, gridDim.x);
+        x_end = share_begin(share, blockIdx.x + 1, gridDim.x);
+        if (x == x_end) return;
+    }
+  do {
+    const int unit = blockIdx.x / cs;
+    int z = 0, h, tile, slot_out = -1;
+    ShareUnit su{};
+    if constexpr (SHARES) {
+        su = share_unit(a, share, x);
+        h = su.head;
+        tile = su.seq;
+    } else {
+        z = unit % a.splits;
+        h = (unit / a.splits) % a.n_kv;
+        // last tiles first: a sequence's later tokens see more keys
+        tile = (int)(gridDim.x / cs / a.splits / a.n_kv) - 1 - unit / a.splits / a.n_kv;
+    }
+    PagedKeys ks;
     PagedTileRows rows;
     if (!paged_tile_rows<ROWS>(a, tile, rows, &ks)) {  // the whole cluster alike
         pdl_wait_prior_grids();
@@ -161,26 +261,40 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     }
 
     const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 4);
-    const int parts = a.splits * cs, part = z * cs + rank;
-    const int b0 = (int)((int64_t)kb.total * part / parts), b1 = (int)((int64_t)kb.total * (part + 1) / parts);
+    int b0, b1;
+    if constexpr (SHARES) {
+        b0 = su.block;
+        b1 = (int)min((int64_t)su.cost, b0 + (x_end - x));
+        if (b0 > 0 || b1 < su.cost) slot_out = b0 > 0 ? 0 : 1;
+        x += b1 - b0;
+        b1 = min(b1, kb.total);
+    } else {
+        const int parts = a.splits * cs, part = z * cs + rank;
+        b0 = (int)((int64_t)kb.total * part / parts);
+        b1 = (int)((int64_t)kb.total * (part + 1) / parts);
+    }
 
     const uint32_t ring = smem_addr(smem) + warp * (U * UNIT);
     const T* const kg = static_cast<const T*>(a.k) + h * a.head_stride;
     const T* const vg = static_cast<const T*>(a.v) + h * a.head_stride;
-    // the page of this lane's key (lanes 0..15) of block i; -2: nobody sees it
-    auto page_of = [&](int i) {
-        if (i >= b1 || lane >= kKeys) return -2;
-        const int j = kb.block(i) * kKeys + lane;
-        return kb.seen(j) ? ks.page(j, a.page_shift) : -2;
+    // this lane's key (lanes 0..15) of block i, where some row sees it
+    auto wanted = [&](int i, int& j) {
+        if (i >= b1 || lane >= kKeys) return false;
+        j = kb.block(i) * kKeys + lane;
+        return kb.seen(j);
     };
-    // where this lane's key of block i begins; -1: zeros
+    auto page_of = [&](int i) {
+        int j;
+        return wanted(i, j) ? ks.page(j, a.page_shift) : 0;
+    };
+    // where the key begins; -1: zeros
     auto offset_of = [&](int i, int page) -> int64_t {
-        if (page == -2) return -1;
+        int j;
+        if (!wanted(i, j)) return -1;
         if ((unsigned)page >= (unsigned)a.n_pages) {
             paged_status(a, VOX_PAGED_BAD_PAGE);
             return -1;
         }
-        const int j = kb.block(i) * kKeys + lane;
         return page * a.page_stride + ks.slot(j, a.page_shift) * a.slot_stride;
     };
     auto issue = [&](const T* base, int64_t off, int slot, bool is_v) {
@@ -492,7 +606,11 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         }
         const int head = head_s[r];
         const float total = tot_s[r];
-        if (a.part_o) {
+        if (SHARES && slot_out >= 0) {
+            const int64_t at = share_slot(blockIdx.x, slot_out, ROWS) + r;
+            if (d == 0) a.part_ml[at] = make_float2(m_s[0][r], total);
+            *reinterpret_cast<float4*>(a.part_o + at * HD + d) = v;
+        } else if (!SHARES && a.part_o) {
             const int64_t at = ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head;
             if (d == 0) a.part_ml[at] = make_float2(m_s[0][r], total);
             *reinterpret_cast<float4*>(a.part_o + at * HD + d) = v;
@@ -502,14 +620,85 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             store4(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + d, v);
         }
     }
+    if (SHARES) __syncthreads();  // the next piece uses the same memory
+  } while (SHARES && x < x_end);
     if (cs > 1) cluster.sync();  // the others may still read this CTA's results
     pdl_wait_prior_grids();      // the launch before this one ends first (PagedAttnArgs::follows)
+}
+
+// Joins the unit that begins in share blockIdx.x and goes on in the next ones.
+template <class T, int HD, int NT>
+__global__ void __launch_bounds__(128) paged_share_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int ROWS = 8 * NT, V4 = HD / 4;
+    __shared__ ShareSums share;
+    const bool some = share_sums(a, share);
+    const int n = gridDim.x, c = blockIdx.x, tid = threadIdx.x;
+    const int64_t x0 = some ? share_begin(share, c, n) : 0, x1 = some ? share_begin(share, c + 1, n) : 0;
+    PagedTileRows rows;
+    PagedKeys ks;
+    ShareUnit u{};
+    bool mine = x1 > x0;
+    if (mine) {
+        u = share_unit(a, share, x1 - 1);
+        mine = u.start >= x0 && u.start + u.cost > x1 && paged_tile_rows<ROWS>(a, u.seq, rows, &ks);
+    }
+    pdl_wait_prior_grids();
+    if (!mine) return;
+    int last = c + 1;
+    while (share_begin(share, last + 1, n) < u.start + u.cost) ++last;
+    for (int i = tid; i < ROWS * V4; i += 128) {
+        const int r = i / V4, d = (i % V4) * 4;
+        const int tok = __shfl_sync(~0u, rows.tok, r), head = u.head * a.group + __shfl_sync(~0u, rows.g, r);
+        if (tok < 0) continue;
+        float top = a.part_ml[share_slot(c, 1, ROWS) + r].x;
+        // (a share without blocks, where there are fewer blocks than shares, wrote nothing)
+        auto empty = [&](int k) { return share_begin(share, k, n) == share_begin(share, k + 1, n); };
+        for (int k = c + 1; k <= last; ++k)
+            if (!empty(k)) top = fmaxf(top, a.part_ml[share_slot(k, 0, ROWS) + r].x);
+        const float base = top == kNegInf ? 0.f : top;
+        float total = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = c; k <= last; ++k) {
+            if (empty(k)) continue;
+            const int64_t at = share_slot(k, k == c, ROWS) + r;
+            const float2 ml = a.part_ml[at];
+            const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
+            const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - base);
+            total = fmaf(f, ml.y, total);
+            v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        store4(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    }
+}
+
+template <class T, int HD, int NT>
+cudaError_t launch_shares(const PagedAttnArgs& a, int shares, cudaStream_t st) {
+    using Cfg = RowsCfg<T, HD, NT>;
+    auto* k = paged_attn_rows_kernel<T, HD, NT, true>;
+    static PagedKernelSetup setup;
+    cudaError_t e = setup(reinterpret_cast<const void*>(k), Cfg::SMEM, false);
+    if (e != cudaSuccess) return e;
+    k<<<shares, 32 * Cfg::WARPS, Cfg::SMEM, st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(shares);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_share_merge_kernel<T, HD, NT>, a);
 }
 
 template <class T, int HD, int NT>
 cudaError_t launch_rows(const PagedAttnArgs& a, int cs, cudaStream_t st) {
     using Cfg = RowsCfg<T, HD, NT>;
-    auto* k = paged_attn_rows_kernel<T, HD, NT>;
+    auto* k = paged_attn_rows_kernel<T, HD, NT, false>;
     static PagedKernelSetup setup;
     cudaError_t e = setup(reinterpret_cast<const void*>(k), Cfg::SMEM, true);
     if (e != cudaSuccess) return e;
@@ -543,7 +732,22 @@ cudaError_t launch_rows_hd(const PagedAttnArgs& a, int nt, int cs, cudaStream_t 
     return a.hd == 128 ? launch_rows_nt<T, 128>(a, nt, cs, st) : launch_rows_nt<T, 64>(a, nt, cs, st);
 }
 
+template <class T>
+cudaError_t launch_shares_hd(const PagedAttnArgs& a, int nt, int shares, cudaStream_t st) {
+    if (a.hd == 128) return nt == 1 ? launch_shares<T, 128, 1>(a, shares, st) : launch_shares<T, 128, 2>(a, shares, st);
+    return nt == 1 ? launch_shares<T, 64, 1>(a, shares, st) : launch_shares<T, 64, 2>(a, shares, st);
+}
+
 }  // namespace
+
+cudaError_t launch_paged_attn_shares(PagedType t, const PagedAttnArgs& a, int nt, int shares, cudaStream_t st) {
+    switch (t) {
+        case PagedType::F32: return launch_shares_hd<float>(a, nt, shares, st);
+        case PagedType::F16: return launch_shares_hd<__half>(a, nt, shares, st);
+        case PagedType::BF16: return launch_shares_hd<__nv_bfloat16>(a, nt, shares, st);
+    }
+    return cudaErrorInvalidValue;
+}
 
 cudaError_t launch_paged_attn_rows(PagedType t, const PagedAttnArgs& a, int nt, int cluster, cudaStream_t st) {
     switch (t) {
