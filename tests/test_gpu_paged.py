@@ -138,20 +138,20 @@ def test_append_reports_bad_pages_and_lengths(V):
 
 # ---- attention ---------------------------------------------------------------
 
-# Batches whose host bounds ask for equal shares of all keys (48 MB and more)
+# Long and short sequences together
 LONG = [
     # dtype, heads, kv, dim, q_len, kv_len, window, sinks
     ("f32", 32, 8, 128, (1,) * 8, (1036, 17, 3000, 0, 1, 900, 16, 257), 0, 0),
     ("bf16", 8, 8, 128, (1, 0, 2, 1, 1) * 3, (1, 5, 2000, 333, 48) * 3, 700, 5),
     ("f16", 16, 8, 64, (2, 1, 8) * 20, (900, 64, 8) * 20, 0, 0),
-    ("bf16", 8, 8, 128, (1,) * 100, (1, 2, 3, 4) * 24 + (800, 1, 1, 0), 0, 0),   # fewer blocks than shares
+    ("bf16", 8, 8, 128, (1,) * 100, (1, 2, 3, 4) * 24 + (800, 1, 1, 0), 0, 0),
     ("bf16", 16, 8, 128, (1,) * 3, (5000, 16, 1), 4500, 40),
 ]
 
 
 @pytest.mark.parametrize("dtype,heads,kv,dim,q_len,kv_len,window,sinks", LONG)
 @pytest.mark.parametrize("prefix", [0, 30])
-def test_decode_in_equal_shares(V, dtype, heads, kv, dim, q_len, kv_len, window, sinks, prefix):
+def test_decode_long_and_short(V, dtype, heads, kv, dim, q_len, kv_len, window, sinks, prefix):
     c = Case(V, torch, dtype, heads, kv, dim, 16, q_len, kv_len, window, sinks, prefix=prefix, seed=25, spare_tokens=2)
     out = torch.full_like(c.q, 3.0)
     c.run(out=out)
@@ -163,7 +163,7 @@ def test_decode_in_equal_shares(V, dtype, heads, kv, dim, q_len, kv_len, window,
     assert torch.equal(out, again)
 
 
-def test_bad_sequences_in_equal_shares(V):
+def test_bad_sequences_among_long_ones(V):
     c = Case(V, torch, "bf16", 8, 8, 128, 16, (1,) * 8, (900, 1600, 30, 700, 1, 1500, 44, 90), seed=26, poison=False)
     want = c.run()
     c.kv[1] = 1601
@@ -176,8 +176,7 @@ def test_bad_sequences_in_equal_shares(V):
         if s in (1, 4):
             assert bool((out[s] == 9.0).all())
         elif s != 5:
-            # shares begin elsewhere: the same terms in another order
-            assert float((out[s] - want[s]).abs().max()) <= 2.0 ** -6 * float(want[s].abs().max())
+            assert torch.equal(out[s], want[s])
     c.q_start.fill_(0)  # no tokens at all
     out.fill_(9.0)
     c.run(out=out)

@@ -215,7 +215,7 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     // equal shares; more, where the bytes bound the call (one decode step's rows),
     // into about four waves, which evens out ragged lengths: 96 sequences of up
     // to 8192 visible keys 411 us against 434 with half as many CTAs.
-    const int64_t slots = 148 * 2;
+    const int64_t slots = 148 * (t == PagedType::F32 && p.nt == 1 ? 3 : 2);
     const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (4 * slots + units - 1) / units : 1;
     // At least 64 keys to a CTA of a cluster (one stream of 1536 tokens: 15 us
     // through clusters alone, 20 us with a merge behind them), 512 where there
@@ -231,7 +231,6 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
 // What a call launches.
 struct AttnPlan {
     KeysPlan own, prefix;
-    int shares = 0;        // > 0: the sequences' keys in so many equal shares
     bool joined = false;   // the prefix as the first part of every sequence's keys
     int parts = 1;         // partial results of a row
     bool partial = false;  // through the workspace
@@ -258,16 +257,6 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
                   (double)b->n_seqs * (double)p->max_len * (double)(c->n_kv_heads * c->head_dim * 2 * type_size(t)) <= 32e6;
     const int64_t keys = visible(b->max_kv_len + (plan.joined ? p->max_len : 0));
     plan.own = plan_keys(c, t, rows, all_rows, keys, [&](int n) { return paged_tiles_bound(a, n); });
-    // Equal shares where the lengths may differ and the keys come from HBM: the
-    // second launch costs about 3 us, from 48 MB on less than the uneven ends.
-    if (plan.own.kernel == KeysPlan::ROWS && rows <= 16 && (!p || plan.joined) && b->n_seqs > 1 &&
-        b->n_seqs <= (size_t)kPagedShareSeqs &&
-        (double)b->n_seqs * (double)keys * (double)(c->n_kv_heads * c->head_dim * 2 * type_size(t)) >= 48e6) {
-        plan.shares = 2 * 148;
-        const size_t slots = (size_t)plan.shares * 2 * 8 * plan.own.nt;
-        plan.ml_bytes = round256(slots * sizeof(float2));
-        plan.bytes = plan.ml_bytes + slots * c->head_dim * sizeof(float);
-    }
     plan.parts = plan.own.splits;
     if (p && !plan.joined) {
         a.keys_of = PagedKeysOf::PREFIX;
@@ -278,8 +267,8 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
     plan.partial = plan.parts > 1;
     if (plan.partial) {
         const size_t n = (size_t)plan.parts * (size_t)all_rows;
-        plan.ml_bytes = std::max(plan.ml_bytes, round256(n * sizeof(float2)));
-        plan.bytes = std::max(plan.bytes, plan.ml_bytes + n * c->head_dim * sizeof(float));
+        plan.ml_bytes = round256(n * sizeof(float2));
+        plan.bytes = plan.ml_bytes + n * c->head_dim * sizeof(float);
     }
     return plan;
 }
@@ -344,7 +333,7 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
         a.pfx_max = (int)p->max_len;
     }
     const AttnPlan plan = plan_attention(c, k.type, b, p, n_heads, window, sinks);
-    if (plan.bytes) {
+    if (plan.partial) {
         if (!ws || ws_bytes < plan.bytes || ((uintptr_t)ws & 255))
             return report_errorf(VOX_ERR_INVALID_ARG, "workspace must be %zu bytes, 256-byte aligned", plan.bytes);
         a.part_ml = static_cast<float2*>(ws);
@@ -357,8 +346,6 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
                          aligned16(a.v, k.type, {}) && aligned16(a.q, k.type, {a.q_ts, a.q_hs}) &&
                          aligned16(a.out, k.type, {a.o_ts, a.o_hs});
     a.keys_of = plan.joined ? PagedKeysOf::JOINED : PagedKeysOf::OWN;
-    if (plan.shares && aligned) return launched(launch_paged_attn_shares(k.type, a, plan.own.nt, plan.shares, st), "paged attention");
-    if (!plan.partial) a.part_o = nullptr, a.part_ml = nullptr;
     const bool shared = p && !plan.joined;
     a.part0 = shared ? plan.prefix.splits : 0;
     TRY(launched(launch_keys(k.type, a, plan.own, aligned, st), "paged attention"));

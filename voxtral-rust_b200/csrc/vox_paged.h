@@ -116,12 +116,6 @@ constexpr int kPagedGeneralRows = 8;  // query rows (token x head of a group) of
 // `cluster` (1..16) CTAs per tile and part.
 cudaError_t launch_paged_attn_rows(PagedType t, const PagedAttnArgs& a, int nt, int cluster, cudaStream_t st);
 
-// The same in equal shares of all sequences' keys (at most one tile of nt (1, 2) x 8
-// rows a sequence), and the launch that joins the shares' pieces.  part_o and
-// part_ml hold 2 slots x nt x 8 rows a share.
-cudaError_t launch_paged_attn_shares(PagedType t, const PagedAttnArgs& a, int nt, int shares, cudaStream_t st);
-constexpr int kPagedShareSeqs = 512;  // most sequences
-
 // tcgen05 attention for many rows per key (vox_paged_tiles.cu): f16 and bf16,
 // head_dim 64 or 128, pages of at least 8 slots, every row on a 16-byte boundary.
 cudaError_t launch_paged_attn_tiles(PagedType t, const PagedAttnArgs& a, cudaStream_t st);

@@ -26,6 +26,7 @@
 #include <cooperative_groups.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "vox_paged.cuh"
 
@@ -37,10 +38,11 @@ namespace {
 
 constexpr int kKeys = 16;
 
-// The ring of a warp holds units of one block's K or V rows, in turn.  16-bit
-// types: 4 warps and 6..8 units of 2..4 KB, two CTAs per SM.  f32 units are 4..8
-// KB: 3 of them with 4 warps for 8 rows (two CTAs per SM), 8 warps in one CTA
-// for more rows, where the tensor cores and not the bytes set the pace.
+// The ring of a warp holds units of one block's K or V rows, in turn; 4 warps.
+// 16-bit types: 6..8 units of 2..4 KB, two CTAs per SM.  f32 units are 4..8 KB,
+// and the arithmetic behind them takes longer than their arrival: two to four
+// units, and with 8 rows three CTAs per SM (eight streams of 1036..3513 tokens 38 us;
+// two CTAs with 3 units a warp 43 us).
 template <class T, int HD, int NT>
 struct RowsCfg {
     static constexpr bool F32 = sizeof(T) == 4;
@@ -49,13 +51,13 @@ struct RowsCfg {
     static constexpr int CHUNKS = ROW_BYTES / 16;
     static constexpr int UNIT = kKeys * ROW_BYTES;
     static constexpr int WARPS = 4;
-    static constexpr int UNITS = F32 ? (HD == 128 ? (NT == 1 ? 3 : 2) : (NT == 4 ? 4 : 6)) : (HD == 128 ? 6 : 8);
+    static constexpr int UNITS = F32 ? (HD == 128 ? 2 : 4) : (HD == 128 ? 6 : 8);
     static constexpr int RING = WARPS * UNITS * UNIT;
     static constexpr int OS = HD + 4;  // row stride of the partial results
     static constexpr int QF = F32 ? HD / 8 * NT * 512 : HD / 32 * NT * 512;
     static constexpr int BODY = RING > WARPS * ROWS * OS * 4 ? RING : WARPS * ROWS * OS * 4;
     static constexpr int SMEM = BODY + QF;
-    static constexpr int PER_SM = SMEM <= 108 * 1024 && WARPS == 4 ? 2 : 1;
+    static constexpr int PER_SM = SMEM <= 72 * 1024 && NT == 1 ? 3 : SMEM <= 108 * 1024 ? 2 : 1;
     static_assert(SMEM <= 216 * 1024, "shared memory");
 };
 
@@ -86,9 +88,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+template <int OFF>
 __device__ __forceinline__ float lds32(uint32_t addr) {
     float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared.f32 %0, [%1 + %2];" : "=f"(v) : "r"(addr), "n"(OFF) : "memory");
     return v;
 }
 
@@ -107,12 +110,26 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo with hi and lo rounded to tf32's 11 bits (half a unit added, the
-// rest cut; the tensor core ignores the low 13 bits of lo itself).  Four
-// full-rate instructions: the conversion instruction runs at a quarter of that.
+// x = hi + lo with hi rounded to tf32's 11 bits (half a unit added, the rest
+// cut), lo the exact rest, of which the tensor core takes 11 bits and ignores the
+// low 13: off by at most 2^-21 of x, 2^-22 where lo is rounded too (the queries
+// and weights, which are split once).  Three full-rate instructions: the
+// conversion instruction runs at a quarter of that.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
-    lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void split_tf32_rounded(float x, uint32_t& hi, uint32_t& lo) {
+    split_tf32(x, hi, lo);
+    lo += 0x1000u;
+}
+template <class F, int... I>
+__device__ __forceinline__ void static_for_each(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F f) {
+    static_for_each(f, std::make_integer_sequence<int, N>{});
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
     const __half2 v = __floats2half2_rn(a, b);
@@ -132,87 +149,7 @@ __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
-// ---- equal shares --------------------------------------------------------------
-//
-// Where sequences of different lengths (at most one tile each) are read from HBM,
-// a CTA takes an equal share of all (sequence, kv head) units' 16-key blocks in
-// one line, instead of a cluster taking a unit: 8 f32 streams of 1036..3513 tokens
-// 43 us with 4 CTAs a unit, 33 us in equal shares.  A share's first piece may end
-// a unit that began in the share before, its last one may begin a unit that goes
-// on: those two are written to the share's slots, and a second launch joins each
-// unit in the share that it begins in.
-
-constexpr int kShareSeqs = kPagedShareSeqs;  // sequences whose running block counts fit
-
-struct ShareSums {
-    int64_t all;               // blocks of all units
-    int sums[kShareSeqs + 1];  // blocks of one kv head of the sequences before
-};
-
-// The block cost of a sequence: at least 1, so that a token that sees nothing is
-// written too; 0 without tokens.
-__device__ __forceinline__ int share_cost(const PagedAttnArgs& a, int s, int plen) {
-    const PagedSeq q = paged_seq(a, s);
-    if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);
-    if (q.nq == 0) return 0;
-    const int len = plen + q.len;
-    return max(1, paged_key_blocks(len - q.nq, len - 1, len, a.window, a.sinks, 4).total);
-}
-
-// All threads of the block call it; false: nothing to do.
-__device__ __forceinline__ bool share_sums(const PagedAttnArgs& a, ShareSums& sh) {
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int plen = a.pfx_len ? paged_prefix_len(a) : 0;
-    if (plen < 0) {
-        if (tid == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
-        return false;
-    }
-    for (int s = tid; s < a.n_seqs; s += blockDim.x) sh.sums[s + 1] = share_cost(a, s, plen);
-    __syncthreads();
-    if (tid < 32) {
-        int before = 0;
-        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-            int n = s0 + lane < a.n_seqs ? sh.sums[s0 + lane + 1] : 0;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(~0u, n, o);
-                if (lane >= o) n += up;
-            }
-            if (s0 + lane < a.n_seqs) sh.sums[s0 + lane + 1] = before + n;
-            before += __shfl_sync(~0u, n, 31);
-        }
-        if (lane == 0) sh.sums[0] = 0, sh.all = (int64_t)before * a.n_kv;
-    }
-    __syncthreads();
-    return sh.all > 0;
-}
-
-// The unit that holds block x of the line, and where in it.
-struct ShareUnit {
-    int seq, head, block, cost;
-    int64_t start;
-};
-__device__ __forceinline__ ShareUnit share_unit(const PagedAttnArgs& a, const ShareSums& sh, int64_t x) {
-    const int want = (int)(x / a.n_kv);
-    int lo = 0, hi = a.n_seqs;  // the last s with sums[s] <= want has a cost above 0
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (sh.sums[mid] <= want) lo = mid; else hi = mid;
-    }
-    ShareUnit u;
-    u.seq = lo;
-    u.cost = sh.sums[lo + 1] - sh.sums[lo];
-    const int64_t r = x - (int64_t)sh.sums[lo] * a.n_kv;
-    u.head = (int)(r / u.cost);
-    u.block = (int)(r - (int64_t)u.head * u.cost);
-    u.start = x - u.block;
-    return u;
-}
-__device__ __forceinline__ int64_t share_begin(const ShareSums& sh, int c, int n) { return sh.all * c / n; }
-
-// The rows' results in a share's slots: [share][slot][row] (m, l) and [.. row][HD].
-__device__ __forceinline__ int64_t share_slot(int share, int slot, int rows) { return ((int64_t)share * 2 + slot) * rows; }
-
-template <class T, int HD, int NT, bool SHARES>
+template <class T, int HD, int NT>
 __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD, NT>::PER_SM)
     paged_attn_rows_kernel(const __grid_constant__ PagedAttnArgs a) {
     using Cfg = RowsCfg<T, HD, NT>;
@@ -228,31 +165,13 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     uint4* qf = reinterpret_cast<uint4*>(smem + Cfg::BODY);
 
     const cg::cluster_group cluster = cg::this_cluster();
-    const int cs = SHARES ? 1 : (int)cluster.num_blocks(), rank = SHARES ? 0 : (int)cluster.block_rank();
+    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     pdl_allow_dependents();
-    __shared__ std::conditional_t<SHARES, ShareSums, char> share;
-    int64_t x = 0, x_end = 0;
-    if constexpr (SHARES) {
-        if (!share_sums(a, share)) return;
-        x = share_begin(share, blockIdx.x, gridDim.x);
-        x_end = share_begin(share, blockIdx.x + 1, gridDim.x);
-        if (x == x_end) return;
-    }
-  do {
     const int unit = blockIdx.x / cs;
-    int z = 0, h, tile, slot_out = -1;
-    ShareUnit su{};
-    if constexpr (SHARES) {
-        su = share_unit(a, share, x);
-        h = su.head;
-        tile = su.seq;
-    } else {
-        z = unit % a.splits;
-        h = (unit / a.splits) % a.n_kv;
-        // last tiles first: a sequence's later tokens see more keys
-        tile = (int)(gridDim.x / cs / a.splits / a.n_kv) - 1 - unit / a.splits / a.n_kv;
-    }
+    const int z = unit % a.splits, h = (unit / a.splits) % a.n_kv;
+    // last tiles first: a sequence's later tokens see more keys
+    const int tile = (int)(gridDim.x / cs / a.splits / a.n_kv) - 1 - unit / a.splits / a.n_kv;
     PagedKeys ks;
     PagedTileRows rows;
     if (!paged_tile_rows<ROWS>(a, tile, rows, &ks)) {  // the whole cluster alike
@@ -261,18 +180,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     }
 
     const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 4);
-    int b0, b1;
-    if constexpr (SHARES) {
-        b0 = su.block;
-        b1 = (int)min((int64_t)su.cost, b0 + (x_end - x));
-        if (b0 > 0 || b1 < su.cost) slot_out = b0 > 0 ? 0 : 1;
-        x += b1 - b0;
-        b1 = min(b1, kb.total);
-    } else {
-        const int parts = a.splits * cs, part = z * cs + rank;
-        b0 = (int)((int64_t)kb.total * part / parts);
-        b1 = (int)((int64_t)kb.total * (part + 1) / parts);
-    }
+    const int parts = a.splits * cs, part = z * cs + rank;
+    const int b0 = (int)((int64_t)kb.total * part / parts), b1 = (int)((int64_t)kb.total * (part + 1) / parts);
 
     const uint32_t ring = smem_addr(smem) + warp * (U * UNIT);
     const T* const kg = static_cast<const T*>(a.k) + h * a.head_stride;
@@ -297,30 +206,39 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         }
         return page * a.page_stride + ks.slot(j, a.page_shift) * a.slot_stride;
     };
-    auto issue = [&](const T* base, int64_t off, int slot, bool is_v) {
-        const uint32_t dst = ring + slot * UNIT;
-        constexpr int RP = 32 / C;  // rows of one pass of the warp
-        const int c = lane % C, r0 = lane / C;
+    // Units go out in the order K, V of the warp's first block, K, V of the next, ...
+    // A block's rows mostly follow one another (one page, all seen): their
+    // addresses are then steps from the first one's, not 16 of their own.
+    constexpr int E = 16 / (int)sizeof(T), RP = 32 / C;  // elements of a copy, rows of one pass of the warp
+    const int cc = lane % C, cr = lane / C;
+    int nxt = b0 + warp, page = page_of(nxt), out_slot = 0;
+    int64_t off = -1, first = 0;
+    bool out_v = false, steps = false;
+    auto issue = [&](const T* base, bool is_v) {
+        const uint32_t dst = ring + out_slot * UNIT;
+        auto to = [&](int r) { return dst + r * Cfg::ROW_BYTES + ((cc ^ (F32 && is_v ? (r & 3) << 1 : r & 7)) << 4); };
+        if (steps) {
+            const T* src = base + first + cr * a.slot_stride + cc * E;
 #pragma unroll
-        for (int n = 0; n < kKeys / RP; ++n) {
-            const int r = n * RP + r0;
-            const int64_t o = __shfl_sync(~0u, off, r);
-            cp16(dst + r * Cfg::ROW_BYTES + ((c ^ (F32 && is_v ? (r & 3) << 1 : r & 7)) << 4),
-                 base + (o >= 0 ? o : 0) + c * (16 / (int)sizeof(T)), o >= 0);
+            for (int n = 0; n < kKeys / RP; ++n, src += RP * a.slot_stride) cp16(to(n * RP + cr), src, true);
+        } else {
+#pragma unroll
+            for (int n = 0; n < kKeys / RP; ++n) {
+                const int64_t o = __shfl_sync(~0u, off, n * RP + cr);
+                cp16(to(n * RP + cr), base + (o >= 0 ? o : 0) + cc * E, o >= 0);
+            }
         }
     };
-    // units go out in the order K, V of the warp's first block, K, V of the next, ...
-    int nxt = b0 + warp, page = page_of(nxt), out_slot = 0;
-    int64_t off = -1;
-    bool out_v = false;
     auto issue_next = [&]() {
         if (nxt < b1) {
             if (!out_v) {
                 off = offset_of(nxt, page);
                 page = page_of(nxt + kWarps);
-                issue(kg, off, out_slot, false);
+                first = __shfl_sync(~0u, off, 0);
+                steps = __all_sync(~0u, lane >= kKeys || (off >= 0 && off == first + lane * a.slot_stride));
+                issue(kg, false);
             } else {
-                issue(vg, off, out_slot, true);
+                issue(vg, true);
             }
         }
         if (out_v) nxt += kWarps;
@@ -336,7 +254,6 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     // Q^T fragments: one 16-byte word per lane and two k steps (f32: hi and lo of one)
     {
         uint32_t* w = reinterpret_cast<uint32_t*>(qf);
-        constexpr int E = 16 / (int)sizeof(T);
         for (int i = tid; i < ROWS * C; i += kThreads) {
             const int r = i / C, c = i % C;
             uint4 v = make_uint4(0, 0, 0, 0);
@@ -348,7 +265,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
                 if constexpr (F32) {
                     const int at = (((c >> 1) * NT + (r >> 3)) * 32 + (r & 7) * 4 + j) * 4 + (c & 1);
                     uint32_t hi, lo;
-                    split_tf32(__uint_as_float(x[j]), hi, lo);
+                    split_tf32_rounded(__uint_as_float(x[j]), hi, lo);
                     w[at] = hi;
                     w[at + 2] = lo;
                 } else {
@@ -382,15 +299,19 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
 
         float s[NT][4] = {}, s2[NT][4] = {}, s3[NT][4] = {};
         if constexpr (F32) {
+            // chunk 2k (+ 1) ^ g: its low 3 bits are one of 8 per lane, the rest a constant
+            const uint32_t at = kt + g * Cfg::ROW_BYTES + t * 4;
+            uint32_t low[8];
 #pragma unroll
-            for (int k = 0; k < HD / 8; ++k) {
-                const uint32_t at = kt + g * Cfg::ROW_BYTES + t * 4;
-                const uint32_t c0 = ((2 * k) ^ g) << 4, c1 = ((2 * k + 1) ^ g) << 4;
+            for (int x = 0; x < 8; ++x) low[x] = at + ((x ^ g) << 4);
+            static_for<HD / 8>([&](auto kc) {
+                constexpr int k = decltype(kc)::value, far = k / 4 * 128, below = 8 * Cfg::ROW_BYTES;
+                const uint32_t c0 = low[2 * k % 8], c1 = low[2 * k % 8 + 1];
                 uint32_t hi[4], lo[4];
-                split_tf32(lds32(at + c0), hi[0], lo[0]);
-                split_tf32(lds32(at + 8 * Cfg::ROW_BYTES + c0), hi[1], lo[1]);
-                split_tf32(lds32(at + c1), hi[2], lo[2]);
-                split_tf32(lds32(at + 8 * Cfg::ROW_BYTES + c1), hi[3], lo[3]);
+                split_tf32(lds32<far>(c0), hi[0], lo[0]);
+                split_tf32(lds32<far + below>(c0), hi[1], lo[1]);
+                split_tf32(lds32<far>(c1), hi[2], lo[2]);
+                split_tf32(lds32<far + below>(c1), hi[3], lo[3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint4 q = qf[(k * NT + n) * 32 + lane];
@@ -398,7 +319,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
                     mma8(s2[n], hi, q.z, q.w);
                     mma8(s[n], hi, q.x, q.y);
                 }
-            }
+            });
         } else {
 #pragma unroll
             for (int k = 0; k < HD / 32; ++k) {
@@ -474,24 +395,28 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
                     for (int x = 0; x < 2; ++x) {  // weight of key t (+ 4) of this half, row g
                         const int src = (t + 4 * x) * 4 + (g >> 1);
                         const float w0 = __shfl_sync(~0u, s[n][2 * k], src), w1 = __shfl_sync(~0u, s[n][2 * k + 1], src);
-                        split_tf32(g & 1 ? w1 : w0, bh[n][x], bl[n][x]);
+                        split_tf32_rounded(g & 1 ? w1 : w0, bh[n][x], bl[n][x]);
                     }
+                // chunk (4 d + g / 4, + 2) ^ 2t: its low 3 bits are one of 4 per lane
+                const uint32_t at = vt + (k * 8 + t) * Cfg::ROW_BYTES + (g & 3) * 4;
+                uint32_t low[4];
 #pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                    const uint32_t at = vt + (k * 8 + t) * Cfg::ROW_BYTES + (g & 3) * 4;
-                    const uint32_t c0 = ((d * 4 + (g >> 2)) ^ (t << 1)) << 4, c1 = ((d * 4 + 2 + (g >> 2)) ^ (t << 1)) << 4;
+                for (int x = 0; x < 4; ++x) low[x] = at + (((2 * x + (g >> 2)) ^ (t << 1)) << 4);
+                static_for<HD / 16>([&](auto dc) {
+                    constexpr int d = decltype(dc)::value, far = d / 2 * 128, below = 4 * Cfg::ROW_BYTES;
+                    const uint32_t c0 = low[2 * (d & 1)], c1 = low[2 * (d & 1) + 1];
                     uint32_t hi[4], lo[4];
-                    split_tf32(lds32(at + c0), hi[0], lo[0]);
-                    split_tf32(lds32(at + c1), hi[1], lo[1]);
-                    split_tf32(lds32(at + 4 * Cfg::ROW_BYTES + c0), hi[2], lo[2]);
-                    split_tf32(lds32(at + 4 * Cfg::ROW_BYTES + c1), hi[3], lo[3]);
+                    split_tf32(lds32<far>(c0), hi[0], lo[0]);
+                    split_tf32(lds32<far>(c1), hi[1], lo[1]);
+                    split_tf32(lds32<far + below>(c0), hi[2], lo[2]);
+                    split_tf32(lds32<far + below>(c1), hi[3], lo[3]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma8(o[d][n], lo, bh[n][0], bh[n][1]);
                         mma8(o[d][n], hi, bl[n][0], bl[n][1]);
                         mma8(o[d][n], hi, bh[n][0], bh[n][1]);
                     }
-                }
+                });
             }
         } else {
             uint32_t b[NT][2];
@@ -606,11 +531,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         }
         const int head = head_s[r];
         const float total = tot_s[r];
-        if (SHARES && slot_out >= 0) {
-            const int64_t at = share_slot(blockIdx.x, slot_out, ROWS) + r;
-            if (d == 0) a.part_ml[at] = make_float2(m_s[0][r], total);
-            *reinterpret_cast<float4*>(a.part_o + at * HD + d) = v;
-        } else if (!SHARES && a.part_o) {
+        if (a.part_o) {
             const int64_t at = ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head;
             if (d == 0) a.part_ml[at] = make_float2(m_s[0][r], total);
             *reinterpret_cast<float4*>(a.part_o + at * HD + d) = v;
@@ -620,85 +541,14 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             store4(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + d, v);
         }
     }
-    if (SHARES) __syncthreads();  // the next piece uses the same memory
-  } while (SHARES && x < x_end);
     if (cs > 1) cluster.sync();  // the others may still read this CTA's results
     pdl_wait_prior_grids();      // the launch before this one ends first (PagedAttnArgs::follows)
-}
-
-// Joins the unit that begins in share blockIdx.x and goes on in the next ones.
-template <class T, int HD, int NT>
-__global__ void __launch_bounds__(128) paged_share_merge_kernel(const __grid_constant__ PagedAttnArgs a) {
-    constexpr int ROWS = 8 * NT, V4 = HD / 4;
-    __shared__ ShareSums share;
-    const bool some = share_sums(a, share);
-    const int n = gridDim.x, c = blockIdx.x, tid = threadIdx.x;
-    const int64_t x0 = some ? share_begin(share, c, n) : 0, x1 = some ? share_begin(share, c + 1, n) : 0;
-    PagedTileRows rows;
-    PagedKeys ks;
-    ShareUnit u{};
-    bool mine = x1 > x0;
-    if (mine) {
-        u = share_unit(a, share, x1 - 1);
-        mine = u.start >= x0 && u.start + u.cost > x1 && paged_tile_rows<ROWS>(a, u.seq, rows, &ks);
-    }
-    pdl_wait_prior_grids();
-    if (!mine) return;
-    int last = c + 1;
-    while (share_begin(share, last + 1, n) < u.start + u.cost) ++last;
-    for (int i = tid; i < ROWS * V4; i += 128) {
-        const int r = i / V4, d = (i % V4) * 4;
-        const int tok = __shfl_sync(~0u, rows.tok, r), head = u.head * a.group + __shfl_sync(~0u, rows.g, r);
-        if (tok < 0) continue;
-        float top = a.part_ml[share_slot(c, 1, ROWS) + r].x;
-        // (a share without blocks, where there are fewer blocks than shares, wrote nothing)
-        auto empty = [&](int k) { return share_begin(share, k, n) == share_begin(share, k + 1, n); };
-        for (int k = c + 1; k <= last; ++k)
-            if (!empty(k)) top = fmaxf(top, a.part_ml[share_slot(k, 0, ROWS) + r].x);
-        const float base = top == kNegInf ? 0.f : top;
-        float total = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int k = c; k <= last; ++k) {
-            if (empty(k)) continue;
-            const int64_t at = share_slot(k, k == c, ROWS) + r;
-            const float2 ml = a.part_ml[at];
-            const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
-            const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - base);
-            total = fmaf(f, ml.y, total);
-            v.x = fmaf(f, o.x, v.x), v.y = fmaf(f, o.y, v.y), v.z = fmaf(f, o.z, v.z), v.w = fmaf(f, o.w, v.w);
-        }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        store4(static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-    }
-}
-
-template <class T, int HD, int NT>
-cudaError_t launch_shares(const PagedAttnArgs& a, int shares, cudaStream_t st) {
-    using Cfg = RowsCfg<T, HD, NT>;
-    auto* k = paged_attn_rows_kernel<T, HD, NT, true>;
-    static PagedKernelSetup setup;
-    cudaError_t e = setup(reinterpret_cast<const void*>(k), Cfg::SMEM, false);
-    if (e != cudaSuccess) return e;
-    k<<<shares, 32 * Cfg::WARPS, Cfg::SMEM, st>>>(a);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(shares);
-    cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_share_merge_kernel<T, HD, NT>, a);
 }
 
 template <class T, int HD, int NT>
 cudaError_t launch_rows(const PagedAttnArgs& a, int cs, cudaStream_t st) {
     using Cfg = RowsCfg<T, HD, NT>;
-    auto* k = paged_attn_rows_kernel<T, HD, NT, false>;
+    auto* k = paged_attn_rows_kernel<T, HD, NT>;
     static PagedKernelSetup setup;
     cudaError_t e = setup(reinterpret_cast<const void*>(k), Cfg::SMEM, true);
     if (e != cudaSuccess) return e;
@@ -732,22 +582,7 @@ cudaError_t launch_rows_hd(const PagedAttnArgs& a, int nt, int cs, cudaStream_t 
     return a.hd == 128 ? launch_rows_nt<T, 128>(a, nt, cs, st) : launch_rows_nt<T, 64>(a, nt, cs, st);
 }
 
-template <class T>
-cudaError_t launch_shares_hd(const PagedAttnArgs& a, int nt, int shares, cudaStream_t st) {
-    if (a.hd == 128) return nt == 1 ? launch_shares<T, 128, 1>(a, shares, st) : launch_shares<T, 128, 2>(a, shares, st);
-    return nt == 1 ? launch_shares<T, 64, 1>(a, shares, st) : launch_shares<T, 64, 2>(a, shares, st);
-}
-
 }  // namespace
-
-cudaError_t launch_paged_attn_shares(PagedType t, const PagedAttnArgs& a, int nt, int shares, cudaStream_t st) {
-    switch (t) {
-        case PagedType::F32: return launch_shares_hd<float>(a, nt, shares, st);
-        case PagedType::F16: return launch_shares_hd<__half>(a, nt, shares, st);
-        case PagedType::BF16: return launch_shares_hd<__nv_bfloat16>(a, nt, shares, st);
-    }
-    return cudaErrorInvalidValue;
-}
 
 cudaError_t launch_paged_attn_rows(PagedType t, const PagedAttnArgs& a, int nt, int cluster, cudaStream_t st) {
     switch (t) {
