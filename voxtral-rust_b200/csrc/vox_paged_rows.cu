@@ -16,7 +16,9 @@
 // mma.m16n8k16 with the weights rounded to the type (half a step of 2^-11 or
 // 2^-8, the size of the result's own rounding); f32 takes mma.m16n8k8 on tf32
 // halves, x = hi + lo with hi and lo rounded to 11 bits each: hi hi + hi lo +
-// lo hi drops lo lo, 2^-22 of the product.
+// lo hi drops lo lo, 2^-22 of the product.  The tensor core cuts its f32 sums
+// instead of rounding them, so f32 sums over the keys are kept outside it: with
+// them inside, results over 2400 keys were 1.7e-6 off instead of 4.7e-7.
 //
 // Work is split over a cluster of up to 16 CTAs per tile, whose partial results
 // meet in distributed shared memory: each CTA joins a slice of the output, in
@@ -111,17 +113,13 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // x = hi + lo with hi rounded to tf32's 11 bits (half a unit added, the rest
-// cut), lo the exact rest, of which the tensor core takes 11 bits and ignores the
-// low 13: off by at most 2^-21 of x, 2^-22 where lo is rounded too (the queries
-// and weights, which are split once).  Three full-rate instructions: the
-// conversion instruction runs at a quarter of that.
+// cut) and lo the exact rest, at most 12 bits that begin 2^-12 below x: the tensor
+// core, which ignores the low 13 bits of a word, takes 11 of them, off by at most
+// 2^-23 of x.  Three full-rate instructions: the conversion instruction runs at a
+// quarter of that.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
-}
-__device__ __forceinline__ void split_tf32_rounded(float x, uint32_t& hi, uint32_t& lo) {
-    split_tf32(x, hi, lo);
-    lo += 0x1000u;
 }
 template <class F, int... I>
 __device__ __forceinline__ void static_for_each(F f, std::integer_sequence<int, I...>) {
@@ -265,7 +263,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
                 if constexpr (F32) {
                     const int at = (((c >> 1) * NT + (r >> 3)) * 32 + (r & 7) * 4 + j) * 4 + (c & 1);
                     uint32_t hi, lo;
-                    split_tf32_rounded(__uint_as_float(x[j]), hi, lo);
+                    split_tf32(__uint_as_float(x[j]), hi, lo);
                     w[at] = hi;
                     w[at + 2] = lo;
                 } else {
@@ -297,7 +295,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         const uint32_t kt = ring + slot * UNIT;
         slot = slot == U - 1 ? 0 : slot + 1;
 
-        float s[NT][4] = {}, s2[NT][4] = {}, s3[NT][4] = {};
+        // f32 with one 8-row group: four sums, so that the products do not queue up
+        float s[NT][4] = {}, s2[NT][4] = {}, s3[4] = {}, s4[4] = {};
         if constexpr (F32) {
             // chunk 2k (+ 1) ^ g: its low 3 bits are one of 8 per lane, the rest a constant
             const uint32_t at = kt + g * Cfg::ROW_BYTES + t * 4;
@@ -315,9 +314,9 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint4 q = qf[(k * NT + n) * 32 + lane];
-                    mma8(s3[n], lo, q.x, q.y);
+                    mma8(NT == 1 ? s3 : s2[n], lo, q.x, q.y);
                     mma8(s2[n], hi, q.z, q.w);
-                    mma8(s[n], hi, q.x, q.y);
+                    mma8(NT == 1 && k % 2 ? s4 : s[n], hi, q.x, q.y);
                 }
             });
         } else {
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                s[n][x] = (s[n][x] + (s2[n][x] + s3[n][x])) * a.scale_log2;
+                s[n][x] = ((s[n][x] + s4[x]) + (s2[n][x] + s3[x])) * a.scale_log2;
                 if (!all && !paged_sees(p[n][x & 1], j0 + g + (x >> 1) * 8, ks.len, a.window, ks.sinks))
                     s[n][x] = kNegInf;
             }
@@ -395,7 +394,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
                     for (int x = 0; x < 2; ++x) {  // weight of key t (+ 4) of this half, row g
                         const int src = (t + 4 * x) * 4 + (g >> 1);
                         const float w0 = __shfl_sync(~0u, s[n][2 * k], src), w1 = __shfl_sync(~0u, s[n][2 * k + 1], src);
-                        split_tf32_rounded(g & 1 ? w1 : w0, bh[n][x], bl[n][x]);
+                        split_tf32(g & 1 ? w1 : w0, bh[n][x], bl[n][x]);
                     }
                 // chunk (4 d + g / 4, + 2) ^ 2t: its low 3 bits are one of 4 per lane
                 const uint32_t at = vt + (k * 8 + t) * Cfg::ROW_BYTES + (g & 3) * 4;
@@ -412,9 +411,12 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
                     split_tf32(lds32<far + below>(c1), hi[3], lo[3]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma8(o[d][n], lo, bh[n][0], bh[n][1]);
-                        mma8(o[d][n], hi, bl[n][0], bl[n][1]);
-                        mma8(o[d][n], hi, bh[n][0], bh[n][1]);
+                        float part[4] = {};
+                        mma8(part, lo, bh[n][0], bh[n][1]);
+                        mma8(part, hi, bl[n][0], bl[n][1]);
+                        mma8(part, hi, bh[n][0], bh[n][1]);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[d][n][x] += part[x];
                     }
                 });
             }
