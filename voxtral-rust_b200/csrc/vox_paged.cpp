@@ -212,14 +212,14 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     p.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
     const int64_t units = std::max<int64_t>(1, tiles(fits ? 8 * p.nt : kPagedGeneralRows) * (int64_t)c->n_kv_heads);
     // CTAs that run at once.  Fewer tiles than that are split into one wave of
-    // equal shares; more, where the bytes bound the call (one decode step's rows),
-    // into about four waves, which evens out ragged lengths: 96 sequences of up
-    // to 8192 visible keys 411 us against 434 with half as many CTAs.
-    const int64_t slots = 148 * (t == PagedType::F32 && p.nt == 1 ? 3 : 2);
-    const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (4 * slots + units - 1) / units : 1;
-    // At least 64 keys to a CTA of a cluster (one stream of 1536 tokens: 15 us
-    // through clusters alone, 20 us with a merge behind them), 512 where there
-    // are enough tiles without, or where the parts go through the merge.
+    // equal parts; more, where the bytes bound the call (one decode step's rows),
+    // into about eight waves, which evens out ragged lengths: 96 sequences of up
+    // to 8192 visible keys 402 us against 408 with two CTAs a tile.
+    const int64_t slots = 148 * (p.nt == 1 ? 3 : 2);
+    const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (8 * slots + units - 1) / units : 1;
+    // At least 64 keys to a CTA of a cluster (one stream of 1536 tokens 9 us through
+    // clusters alone, 14 us with a merge behind them), 512 where there are enough
+    // tiles without, or where the parts go through the merge.
     int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / (units < slots ? 64 : 512)));
     if (fits)
         while (p.cluster < 16 && 2 * p.cluster <= parts) p.cluster *= 2;

@@ -41,10 +41,10 @@ namespace {
 constexpr int kKeys = 16;
 
 // The ring of a warp holds units of one block's K or V rows, in turn; 4 warps.
-// 16-bit types: 6..8 units of 2..4 KB, two CTAs per SM.  f32 units are 4..8 KB,
-// and the arithmetic behind them takes longer than their arrival: two to four
-// units, and with 8 rows three CTAs per SM (eight streams of 1036..3513 tokens 38 us;
-// two CTAs with 3 units a warp 43 us).
+// With 8 rows three CTAs share an SM, so that one's start and end lie under the
+// others' copies (96 ragged f16 sequences 417 us with two CTAs of 6 units a warp,
+// 402 us with three of 4; eight f32 streams 43 and 38 us); with more rows the
+// registers allow two.
 template <class T, int HD, int NT>
 struct RowsCfg {
     static constexpr bool F32 = sizeof(T) == 4;
@@ -53,7 +53,7 @@ struct RowsCfg {
     static constexpr int CHUNKS = ROW_BYTES / 16;
     static constexpr int UNIT = kKeys * ROW_BYTES;
     static constexpr int WARPS = 4;
-    static constexpr int UNITS = F32 ? (HD == 128 ? 2 : 4) : (HD == 128 ? 6 : 8);
+    static constexpr int UNITS = F32 ? (HD == 128 ? 2 : 4) : (HD == 128 ? (NT == 1 ? 4 : 6) : 8);
     static constexpr int RING = WARPS * UNITS * UNIT;
     static constexpr int OS = HD + 4;  // row stride of the partial results
     static constexpr int QF = F32 ? HD / 8 * NT * 512 : HD / 32 * NT * 512;
