@@ -13,9 +13,10 @@ namespace {
 // tokens by latency.  A thread owns one 16-byte column of a token's rows: its
 // pairs' sines and cosines are computed once, then it walks over the heads of k, v
 // and q with up to 6 rows in flight, loaded before it is known where the token
-// goes.  A CTA of 256 threads takes 4 tokens where there are many (fewer sines,
-// more bytes in flight per CTA: 8.8k tokens 81 -> 65 us), one where there are few
-// (all heads at once).
+// goes.  A CTA of 256 threads takes 2 tokens where there are many (fewer sines; one
+// round of loads for 32 + 16 heads of 128: 8.8k tokens 59 us, 4.3 TB/s, against 62
+// with 4 tokens and two rounds, 81 with one), and one where there are few (all
+// heads at once: a single token 3.4 us in a graph).
 //
 // The angle a * theta^(-2c/D) matters modulo a turn only.  turns[c] is the turn
 // fraction per position as a 64-bit binary fraction, so the 64-bit product with
@@ -88,7 +89,7 @@ __device__ __forceinline__ AppendPlace append_place(const PagedAppendArgs& a, in
 }
 
 template <class T, bool WIDE, int TOKENS>
-__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
+__global__ void __launch_bounds__(256, 4) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
     constexpr int N = AppendUnit<T, WIDE>::N, P = N / 2, U = TOKENS > 1 ? 6 : 4, TT = 256 / TOKENS;
     const int chunks = a.hd / N, heads_at_once = TT / chunks;
     const int tid = threadIdx.x % TT;
@@ -377,9 +378,9 @@ cudaError_t by_type(PagedType t, F f) {
 cudaError_t launch_paged_append(PagedType t, const PagedAppendArgs& a, bool wide, cudaStream_t st) {
     return by_type(t, [&](auto x) {
         using T = decltype(x);
-        // 4 tokens to a CTA once that still leaves two CTAs to every SM
-        if (wide && a.n_tokens >= 4 * 296)
-            paged_append_kernel<T, true, 4><<<(a.n_tokens + 3) / 4, 256, 0, st>>>(a);
+        // 2 tokens to a CTA once that still leaves four CTAs to every SM
+        if (wide && a.n_tokens >= 2 * 4 * 148)
+            paged_append_kernel<T, true, 2><<<(a.n_tokens + 1) / 2, 256, 0, st>>>(a);
         else if (wide)
             paged_append_kernel<T, true, 1><<<a.n_tokens, 256, 0, st>>>(a);
         else
