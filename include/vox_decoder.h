@@ -569,7 +569,10 @@ int vox_attention_gqa_step_noalloc(const float* d_query, const float* d_keys,
  * these calls is DEVICE memory the caller owns (on `device` of the cache);
  * the calls are asynchronous on `stream` (a cudaStream_t, 0 = default
  * stream), allocate nothing, keep nothing between calls, may be captured into
- * a graph, and leave the calling thread's current device as it was.  All
+ * a graph, and leave the calling thread's current device as it was.  A CUDA
+ * error already pending on the calling thread is reported as VOX_ERR_CUDA and
+ * nothing is launched.  (What a call keeps is that a kernel's limits have been
+ * raised on a device: not after cudaDeviceReset.)  All
  * tensors of a call have the cache's dtype: VOX_DT_F32, VOX_DT_F16 or
  * VOX_DT_BF16.  Strides are in elements.
  *
@@ -633,20 +636,22 @@ int vox_paged_append_rope(const vox_paged_cache* cache, const vox_paged_batch* b
  * Keys and values that a token does not see do not affect it, whatever they
  * hold; page ids that no token needs are not looked at.  scale 0 =
  * 1/sqrt(head_dim).  f16 and bf16 tensors are multiplied as they are and
- * accumulated in f32.  `workspace` is scratch memory of the size that
- * vox_paged_attention_workspace gives (it may be 0), 256-byte aligned; calls
- * that can overlap on the GPU need one each. */
+ * accumulated in f32.  `out` must not overlap q or the pool.  `workspace` is
+ * scratch memory of the size that vox_paged_attention_workspace gives (it may
+ * be 0), 256-byte aligned; calls that can overlap on the GPU need one each. */
 int vox_paged_attention_workspace(const vox_paged_cache* cache, const vox_paged_batch* batch, size_t n_heads,
                                   size_t sliding_window, size_t n_sinks, size_t* bytes);
 int vox_paged_attention(const vox_paged_cache* cache, const vox_paged_batch* batch, const vox_rows* q,
                         size_t n_heads, size_t sliding_window, size_t n_sinks, float scale, const vox_rows* out,
                         void* workspace, size_t workspace_bytes, void* stream);
 /* The same for a batch whose sequences all begin with one shared prefix,
- * which is read and multiplied once for all of them: *prefix_len tokens (a
- * device int32, at most max_prefix_len) in the pages prefix_pages
- * [n_prefix_pages].  The batch's table, kv_len and bounds are those of the
- * sequences' own tokens behind the prefix; a token's index, for the window
- * and the sinks, is *prefix_len + its index among its sequence's own. */
+ * which is read from memory once for all of them (and multiplied once, unless
+ * it is so short that reading it out of the L2 for every sequence is faster):
+ * *prefix_len tokens (a device int32, at most max_len) in the pages
+ * prefix->pages [n_pages].  The batch's table, kv_len and bounds are those of
+ * the sequences' own tokens behind the prefix; a token's index, for the window
+ * and the sinks, is the prefix's length + its index among its sequence's own.  A
+ * length out of bounds skips the call and sets VOX_PAGED_BAD_LENGTH. */
 typedef struct vox_paged_prefix {
     const int32_t* pages;
     const int32_t* len;

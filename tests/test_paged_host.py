@@ -12,6 +12,9 @@ def V():
     return vox()
 
 
+OUT = 1 << 21  # another made-up address: results must not replace their queries
+
+
 def descs(V, **kw):
     """A valid cache, batch, prefix and row set on made-up addresses (never read here)."""
     a = 1 << 20
@@ -113,6 +116,13 @@ def test_rows_are_checked(V):
         refused(V, L.vox_paged_append_rope(c, b, r, r, 1e4, 4, r, bad, None), code, word)
 
 
+def test_results_must_not_replace_the_queries(V):
+    c, b, p, r = (C.byref(x) for x in descs(V))
+    L = V.lib()
+    refused(V, L.vox_paged_attention(c, b, r, 4, 0, 0, 0.0, r, None, 0, None), "ERR_INVALID_ARG", "out must not be q")
+    refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 0.0, r, None, 0, None), "ERR_INVALID_ARG", "out must not be q")
+
+
 def test_prefix_is_checked(V):
     L = V.lib()
     for change, code in ((dict(len=None), "ERR_INVALID_ARG"), (dict(pages=None), "ERR_INVALID_ARG"),
@@ -134,9 +144,10 @@ def test_workspace_is_asked_for(V):
     """A prefix long enough to be read once for all sequences leaves partial results."""
     c, b, p, r = (C.byref(x) for x in descs(V, prefix=dict(n_pages=2100, max_len=33000)))
     L, n = V.lib(), C.c_size_t()
+    o = C.byref(descs(V, rows=dict(ptr=OUT))[3])
     assert L.vox_paged_prefix_attention_workspace(c, b, p, 4, 0, 0, C.byref(n)) == 0 and n.value > 0
-    refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 0.0, r, None, 0, None), "ERR_INVALID_ARG", "workspace")
-    refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 0.0, r, (1 << 20) + 8, 1 << 30, None),
+    refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 0.0, o, None, 0, None), "ERR_INVALID_ARG", "workspace")
+    refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 0.0, o, (1 << 20) + 8, 1 << 30, None),
             "ERR_INVALID_ARG", "workspace")
 
 

@@ -319,6 +319,7 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
     a.v = c->values;
     TRY(check_rows(q, "q", b->n_tokens, n_heads, c->head_dim, k.type, false, &a.q_ts, &a.q_hs));
     TRY(check_rows(out, "out", b->n_tokens, n_heads, c->head_dim, k.type, true, &a.o_ts, &a.o_hs));
+    if (q->ptr == out->ptr) return report_errorf(VOX_ERR_INVALID_ARG, "out must not be q");
     a.q = q->ptr;
     a.out = out->ptr;
     a.n_heads = (int)n_heads;
