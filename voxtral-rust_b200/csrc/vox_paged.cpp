@@ -217,9 +217,9 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     // to 8192 visible keys 402 us against 408 with two CTAs a tile.
     const int64_t slots = 148 * (p.nt == 1 ? 3 : 2);
     const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (8 * slots + units - 1) / units : 1;
-    // At least 64 keys to a CTA of a cluster (one stream of 1536 tokens 9 us through
-    // clusters alone, 14 us with a merge behind them), 512 where there are enough
-    // tiles without, or where the parts go through the merge.
+    // At least 64 keys to a CTA of a cluster, 512 where there are enough tiles
+    // without, or where the parts go through the merge (one stream of 1536 tokens:
+    // 15 us a call through clusters alone, 20 us with a merge behind them).
     int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / (units < slots ? 64 : 512)));
     if (fits)
         while (p.cluster < 16 && 2 * p.cluster <= parts) p.cluster *= 2;
@@ -242,7 +242,7 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
     AttnPlan plan;
     const int64_t group = (int64_t)(n_heads / c->n_kv_heads), all_rows = (int64_t)(b->n_tokens * n_heads);
     auto visible = [&](size_t len) {
-        return (int64_t)(window ? std::min(len, window + b->max_q_len + std::min(sinks, len)) : len);
+        return (int64_t)(window && window < len ? std::min(len, window + b->max_q_len + std::min(sinks, len)) : len);
     };
     PagedAttnArgs a{};
     a.n_tokens = (int)b->n_tokens;

@@ -15,8 +15,8 @@
 // tcgen05 has no use here: its smallest tile has 64 rows.  f16 and bf16 take
 // mma.m16n8k16 with the weights rounded to the type (half a step of 2^-11 or
 // 2^-8, the size of the result's own rounding); f32 takes mma.m16n8k8 on tf32
-// halves, x = hi + lo with hi and lo rounded to 11 bits each: hi hi + hi lo +
-// lo hi drops lo lo, 2^-22 of the product.  The tensor core cuts its f32 sums
+// halves, x = hi + lo with hi rounded to 11 bits: hi hi + hi lo + lo hi drops lo
+// lo, 2^-22 of the product.  The tensor core cuts its f32 sums
 // instead of rounding them, so f32 sums over the keys are kept outside it: with
 // them inside, results over 2400 keys were 1.7e-6 off instead of 4.7e-7.
 //
@@ -43,8 +43,8 @@ constexpr int kKeys = 16;
 // The ring of a warp holds units of one block's K or V rows, in turn; 4 warps.
 // With 8 rows three CTAs share an SM, so that one's start and end lie under the
 // others' copies (96 ragged f16 sequences 417 us with two CTAs of 6 units a warp,
-// 402 us with three of 4; eight f32 streams 43 and 38 us); with more rows the
-// registers allow two.
+// 402 us with three of 4; eight f32 streams 43 us with two of 3, 38 us with three of
+// 2); with more rows the registers allow two.
 template <class T, int HD, int NT>
 struct RowsCfg {
     static constexpr bool F32 = sizeof(T) == 4;
