@@ -287,6 +287,9 @@ int check_attention(const vox_paged_cache* c, const vox_paged_batch* b, const vo
     TRY(check_batch(c, b));
     if (n_heads == 0 || n_heads > 65536 || n_heads % c->n_kv_heads)
         return report_errorf(VOX_ERR_INVALID_ARG, "n_heads must be > 0 and divisible by n_kv_heads");
+    // the kernels count query rows, rounded up to whole tiles, in 32 bits
+    if ((b->n_tokens + 256) * n_heads > kMaxCount * 2)
+        return report_errorf(VOX_ERR_UNSUPPORTED, "n_tokens * n_heads must be at most %d", (int)(kMaxCount * 2));
     if (p) {
         if (!p->len || (p->n_pages && !p->pages)) return report_errorf(VOX_ERR_INVALID_ARG, "null prefix pages or length");
         if (p->n_pages > kMaxCount || p->max_len > kMaxCount)

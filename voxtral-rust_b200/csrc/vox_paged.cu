@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(kGenThreads) paged_attn_general_kernel(const _
         q_s[i] = x;
     }
     const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 5);
-    const int b0 = (int)((int64_t)kb.total * z / a.splits), b1 = (int)((int64_t)kb.total * (z + 1) / a.splits);
+    int b0, b1;
+    paged_part(kb.total, z, a.splits, &b0, &b1);
 
     float acc[R][2] = {};
     float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};  // rows warp and warp + 4
@@ -300,9 +301,9 @@ template <class T, int V>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttnArgs a, int n_parts) {
     constexpr int E = V ? V : kPagedMaxHeadDim / 32;
     const int64_t n_rows = (int64_t)a.n_tokens * a.n_heads;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    const int tok = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
+    const int tok = row / a.n_heads, head = row % a.n_heads;
     bool mine = row < n_rows && !(a.pfx_len && paged_prefix_len(a) < 0);
     if (mine) {
         const int s = paged_seq_of_warp(a, tok);

@@ -77,7 +77,7 @@ __device__ __forceinline__ int paged_prefix_len(const PagedAttnArgs& a) {
 // sequence (-1: none) and the tile's place in it.
 __device__ __forceinline__ int paged_find_tile(const PagedAttnArgs& a, int t, int rows, int* place) {
     const int lane = threadIdx.x & 31;
-    if ((int64_t)a.max_q * a.group <= rows) {  // at most one tile a sequence
+    if (a.max_q * a.group <= rows) {  // at most one tile a sequence
         *place = 0;
         return t < a.n_seqs ? t : -1;
     }
@@ -88,7 +88,7 @@ __device__ __forceinline__ int paged_find_tile(const PagedAttnArgs& a, int t, in
         if (s < a.n_seqs) {
             const PagedSeq q = paged_seq(a, s);
             if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);  // no tile stands for it
-            n = (int)(((int64_t)q.nq * a.group + rows - 1) / rows);
+            n = (q.nq * a.group + rows - 1) / rows;
         }
         int sum = n;
         for (int o = 1; o < 32; o <<= 1) {
@@ -128,6 +128,13 @@ __device__ __forceinline__ KeyBlocks paged_key_blocks(int pmin, int pmax, int le
     b.first = max(b.lo >> shift, b.sink_blocks);
     b.total = b.sink_blocks + max(0, nb - b.first);
     return b;
+}
+
+// The blocks [begin, end) of part `part` of `parts` equal ones of `total`.
+__device__ __forceinline__ void paged_part(int total, int part, int parts, int* begin, int* end) {
+    const int each = total / parts, more = total - each * parts;
+    *begin = each * part + min(part, more);
+    *end = *begin + each + (part < more);
 }
 
 // Whether the token with index p sees key j (of keys 0..len-1).
@@ -205,7 +212,7 @@ __device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile
         return false;
     }
     rows.tok = rows.p = -1;
-    int64_t row;
+    int row;  // (the host has checked that tokens x heads fit 32 bits)
     ks->pfx = nullptr;
     ks->plen = 0;
     if (a.keys_of != PagedKeysOf::PREFIX) {
@@ -215,9 +222,9 @@ __device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile
         const PagedSeq q = paged_seq(a, s);
         if (!q.ok && threadIdx.x == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
         if (q.nq == 0) return false;
-        row = (int64_t)place * ROWS + lane;
-        if (lane < ROWS && row < (int64_t)q.nq * a.group) {
-            const int i = (int)(row / a.group);
+        row = place * ROWS + lane;
+        if (lane < ROWS && row < q.nq * a.group) {
+            const int i = row / a.group;
             rows.tok = q.q0 + i;
             rows.p = q.len - q.nq + i;
         }
@@ -233,9 +240,9 @@ __device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile
             ks->sinks = max(0, a.sinks - plen);
         }
     } else {
-        row = (int64_t)tile * ROWS + lane;
-        if (lane < ROWS && row < (int64_t)a.n_tokens * a.group) {
-            const int t = (int)(row / a.group);
+        row = tile * ROWS + lane;
+        if (lane < ROWS && row < a.n_tokens * a.group) {
+            const int t = row / a.group;
             const int s = paged_seq_of(a, t);
             if (s >= 0) {
                 const PagedSeq q = paged_seq(a, s);
@@ -247,7 +254,7 @@ __device__ __forceinline__ bool paged_tile_rows(const PagedAttnArgs& a, int tile
         ks->len = plen;
         ks->sinks = a.sinks;
     }
-    rows.g = (int)(row % a.group);
+    rows.g = row % a.group;
     rows.pmin = __reduce_min_sync(~0u, rows.tok >= 0 ? rows.p : 0x7FFFFFFF);
     rows.pmax = __reduce_max_sync(~0u, rows.tok >= 0 ? rows.p : -0x7FFFFFFF);
     return rows.pmin <= rows.pmax;

@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     }
 
     const KeyBlocks kb = paged_key_blocks(rows.pmin, rows.pmax, ks.len, a.window, ks.sinks, 4);
-    const int parts = a.splits * cs, part = z * cs + rank;
-    const int b0 = (int)((int64_t)kb.total * part / parts), b1 = (int)((int64_t)kb.total * (part + 1) / parts);
+    int b0, b1;
+    paged_part(kb.total, z * cs + rank, a.splits * cs, &b0, &b1);
 
     const uint32_t ring = smem_addr(smem) + warp * (U * UNIT);
     const T* const kg = static_cast<const T*>(a.k) + h * a.head_stride;

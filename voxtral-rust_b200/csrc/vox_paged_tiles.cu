@@ -302,24 +302,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ks.table = a.table + seq * a.table_stride;
         ks.len = q.len;
         ks.sinks = max(0, a.sinks - plen);
-        const int64_t row = (int64_t)place * (2 * kTile) + tid;
-        if (tid < 2 * kTile && row < (int64_t)q.nq * a.group) {
-            const int i = (int)(row / a.group);
+        const int row = place * (2 * kTile) + tid;
+        if (tid < 2 * kTile && row < q.nq * a.group) {
+            const int i = row / a.group;
             tok = q.q0 + i;
             p = q.len - q.nq + i;
-            head = h * a.group + (int)(row - (int64_t)i * a.group);
+            head = h * a.group + row - i * a.group;
         }
     } else {
-        const int64_t row = (int64_t)tile * (2 * kTile) + tid;
-        if (tid < 2 * kTile && row < (int64_t)a.n_tokens * a.group) {
-            const int t = (int)(row / a.group), s = paged_seq_of(a, t);
+        const int row = tile * (2 * kTile) + tid;
+        if (tid < 2 * kTile && row < a.n_tokens * a.group) {
+            const int t = row / a.group, s = paged_seq_of(a, t);
             if (s >= 0) {
                 const PagedSeq q = paged_seq(a, s);
                 if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);
                 if (t - q.q0 < q.nq) {
                     tok = t;
                     p = plen + q.len - q.nq + (t - q.q0);
-                    head = h * a.group + (int)(row - (int64_t)t * a.group);
+                    head = h * a.group + row - t * a.group;
                 }
             }
         }
@@ -376,8 +376,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     const bool any = pmin <= pmax;
     const KeyBlocks kb = paged_key_blocks(pmin, pmax, ks.len, a.window, ks.sinks, 7);
-    const int b0 = any ? (int)((int64_t)kb.total * z / a.splits) : 0;
-    const int n = any ? (int)((int64_t)kb.total * (z + 1) / a.splits) - b0 : 0;
+    int b0 = 0, n = 0;
+    if (any) {
+        paged_part(kb.total, z, a.splits, &b0, &n);
+        n -= b0;
+    }
 
     if (warp == 10) {
         // ---- K and V tiles ----
