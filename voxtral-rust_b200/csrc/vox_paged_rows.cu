@@ -272,11 +272,6 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             }
         }
     }
-    int p[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) p[n][e] = __shfl_sync(~0u, rows.p, n * 8 + 2 * t + e);
     if (tid < ROWS) tok_s[tid] = rows.tok, head_s[tid] = h * a.group + rows.g, p_s[tid] = rows.p;
 
     __syncthreads();
@@ -347,7 +342,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 s[n][x] = ((s[n][x] + s4[x]) + (s2[n][x] + s3[x])) * a.scale_log2;
-                if (!all && !paged_sees(p[n][x & 1], j0 + g + (x >> 1) * 8, ks.len, a.window, ks.sinks))
+                if (!all && !paged_sees(p_s[n * 8 + 2 * t + (x & 1)], j0 + g + (x >> 1) * 8, ks.len, a.window, ks.sinks))
                     s[n][x] = kNegInf;
             }
 #pragma unroll
