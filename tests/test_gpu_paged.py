@@ -367,6 +367,16 @@ def test_shared_prefix(V, dtype, heads, kv, dim, prefix, q_len, kv_len, window, 
     assert int(c.status) == 0
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("prefix,page", [(1, 256), (300, 64), (128, 128)])
+def test_prefix_that_no_window_reaches(V, dtype, prefix, page):
+    """Its pages (-1 in the list) are not looked at."""
+    c = Case(V, torch, dtype, 14, 2, 128, page, (64, 50), (155, 97), 5, 0, prefix=prefix, seed=27)
+    assert (c.pre == -1).all()
+    c.check(c.run())
+    assert int(c.status) == 0
+
+
 def test_bad_shared_prefix_is_reported(V):
     c = Case(V, torch, "bf16", 8, 2, 128, 16, (1,) * 40, (5,) * 40, prefix=1200, seed=24)
     want = c.run()

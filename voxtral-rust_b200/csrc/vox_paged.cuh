@@ -114,6 +114,8 @@ struct KeyBlocks {
     int end, lo, sinks;             // keys [0, min(sinks, end)) and [lo, end) are seen
     __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : first + i - sink_blocks; }
     __device__ __forceinline__ bool seen(int j) const { return j < end && (j >= lo || j < sinks); }
+    // whether any of the n keys from j on is
+    __device__ __forceinline__ bool any_seen(int j, int n) const { return max(j, lo) < min(j + n, end) || j < min(sinks, end); }
 };
 __device__ __forceinline__ KeyBlocks paged_key_blocks(int pmin, int pmax, int len, int window, int sinks, int shift) {
     KeyBlocks b;
@@ -126,7 +128,7 @@ __device__ __forceinline__ KeyBlocks paged_key_blocks(int pmin, int pmax, int le
     const int se = min(b.sinks, b.end);
     b.sink_blocks = (se >> shift) + ((se & mask) != 0);
     b.first = max(b.lo >> shift, b.sink_blocks);
-    b.total = b.sink_blocks + max(0, nb - b.first);
+    b.total = b.sink_blocks + (b.lo < b.end ? max(0, nb - b.first) : 0);
     return b;
 }
 

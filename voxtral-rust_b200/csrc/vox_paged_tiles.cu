@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             __syncwarp();
             if (lane < boxes) {
                 const int j = j0 + lane * box;
-                bool seen = j < kb.end && (j + box > kb.lo || j < kb.sinks);
+                bool seen = kb.any_seen(j, box);
                 int page = seen ? ks.table[j >> a.page_shift] : -1;
                 if (seen && (unsigned)page >= (unsigned)a.n_pages) {
                     paged_status(a, VOX_PAGED_BAD_PAGE);
