@@ -214,6 +214,28 @@ def test_prefill_ragged(V, dtype, heads, kv, dim, window, sinks):
     assert int(c.status) == 0
 
 
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f16", 128)])
+@pytest.mark.parametrize("window,sinks,longest", [(0, 0, 1500), (600, 4, 1500)])
+def test_a_last_wave_of_few_tiles(V, dtype, dim, window, sinks, longest):
+    """152 tiles of 256 rows: 148 as they are, the last 4 in parts."""
+    q_len = tuple(65 - (i % 3 == 1) for i in range(19))
+    kv_len = tuple(longest - 70 * i for i in range(19))
+    c = Case(V, torch, dtype, 16, 4, dim, 16, q_len, kv_len, window, sinks, seed=28, spare_tokens=5)
+    c.v[18][kv_len[18] - 1, 0, 3] = math.nan  # seen by the last token alone, in a split tile or not
+    c.vp[c.table[18, (kv_len[18] - 1) // 16], 0, (kv_len[18] - 1) % 16, 3] = math.nan
+    c.v[0][longest - 1, 1, 5] = math.inf
+    c.vp[c.table[0, (longest - 1) // 16], 1, (longest - 1) % 16, 5] = math.inf
+    out = torch.full_like(c.q, 3.0)
+    c.run(out=out)
+    assert bool((out[sum(q_len):] == 3.0).all()) and int(c.status) == 0
+    want, tol = c.expected()
+    got = out.float().cpu().numpy()[:sum(q_len)]
+    want, tol = want[:sum(q_len)], tol[:sum(q_len)]
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
+    ok = np.isfinite(want)
+    assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+
+
 @pytest.mark.parametrize("layout", ["heads", "slots", "pair"])
 @pytest.mark.parametrize("dim,page", [(128, 16), (64, 128), (64, 8)])
 @pytest.mark.parametrize("q_len,kv_len", [((1, 1), (77, 300)), ((120, 65), (400, 65))])

@@ -180,12 +180,14 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 struct KeysPlan {
     enum Kernel { GENERAL, ROWS, TILES } kernel = GENERAL;
     int nt = 1, cluster = 1, splits = 1;
+    int whole = -1, units = 0;  // TILES: see PagedAttnArgs::whole
 };
 
 // `rows`: query rows that share their keys (a sequence's, or all); `all_rows`:
-// tokens x heads; `tiles(n)`: tiles of n rows; `keys`: keys that a row can see.
+// tokens x heads; `tiles(n)`: tiles of n rows; `keys`: keys that a row can see;
+// `alike`: no merge follows anyway, and the tiles see about as many keys each.
 template <class F>
-KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t all_rows, int64_t keys, F tiles) {
+KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t all_rows, int64_t keys, bool alike, F tiles) {
     KeysPlan p;
     const bool fits = c->head_dim == 64 || c->head_dim == 128;
     // tcgen05 tiles have 128 rows: from 32 rows on they win although part of
@@ -205,6 +207,15 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
             if (z > 1 && units >= 3 * 148) break;
             const double t = (double)((units * z + 147) / 148) * (double)((blocks + z - 1) / z + 3) + (z > 1 ? part * (double)z : 0.0);
             if (z == 1 || t < best) best = t, p.splits = (int)z;
+        }
+        // A last wave that leaves at least half of the SMs empty: only its tiles are
+        // split, over all SMs (512 tiles of 65 blocks, 3.46 waves: 487 us instead of
+        // 528); joining them costs about 2 blocks' time.
+        const int64_t last = units % 148;
+        if (alike && units > 148 && last > 0 && last <= 74) {
+            const int64_t z = std::min<int64_t>(148 / last, blocks / 2);
+            const double t2 = (double)(units / 148) * (double)(blocks + 3) + (double)((blocks + z - 1) / std::max<int64_t>(z, 1) + 5);
+            if (z > 1 && t2 < best) p.splits = (int)z, p.whole = (int)(units - last), p.units = (int)units;
         }
         return p;
     }
@@ -256,17 +267,20 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
     plan.joined = p && rows <= 32 &&
                   (double)b->n_seqs * (double)p->max_len * (double)(c->n_kv_heads * c->head_dim * 2 * type_size(t)) <= 32e6;
     const int64_t keys = visible(b->max_kv_len + (plan.joined ? p->max_len : 0));
-    plan.own = plan_keys(c, t, rows, all_rows, keys, [&](int n) { return paged_tiles_bound(a, n); });
+    // a long past or a window in front of few new tokens
+    const bool alike = !p && keys >= 3 * (int64_t)b->max_q_len;
+    plan.own = plan_keys(c, t, rows, all_rows, keys, alike, [&](int n) { return paged_tiles_bound(a, n); });
     plan.parts = plan.own.splits;
     if (p && !plan.joined) {
         a.keys_of = PagedKeysOf::PREFIX;
-        plan.prefix = plan_keys(c, t, (int64_t)b->n_tokens * group, all_rows, visible(p->max_len),
+        plan.prefix = plan_keys(c, t, (int64_t)b->n_tokens * group, all_rows, visible(p->max_len), false,
                                 [&](int n) { return paged_tiles_bound(a, n); });
         plan.parts += plan.prefix.splits;
     }
     plan.partial = plan.parts > 1;
     if (plan.partial) {
-        const size_t n = (size_t)plan.parts * (size_t)all_rows;
+        const size_t n = plan.own.whole >= 0 ? (size_t)(plan.own.units - plan.own.whole) * plan.own.splits * kPagedTileRows
+                                             : (size_t)plan.parts * (size_t)all_rows;
         plan.ml_bytes = round256(n * sizeof(float2));
         plan.bytes = plan.ml_bytes + n * c->head_dim * sizeof(float);
     }
@@ -275,8 +289,13 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
 
 cudaError_t launch_keys(PagedType t, PagedAttnArgs& a, const KeysPlan& p, bool aligned, cudaStream_t st) {
     a.splits = p.splits;
-    if (p.kernel == KeysPlan::TILES && aligned && std::max({a.page_stride, a.head_stride, a.slot_stride}) < (int64_t(1) << 39))
+    a.whole = -1;
+    if (p.kernel == KeysPlan::TILES && aligned && std::max({a.page_stride, a.head_stride, a.slot_stride}) < (int64_t(1) << 39)) {
+        a.whole = p.whole;
         return launch_paged_attn_tiles(t, a, st);
+    }
+    // (no room in the workspace for parts of all rows where only the last tiles' was planned)
+    if (p.whole >= 0) a.splits = 1, a.part_o = nullptr, a.part_ml = nullptr;
     if (p.kernel == KeysPlan::ROWS && aligned) return launch_paged_attn_rows(t, a, p.nt, p.cluster, st);
     return launch_paged_attn_general(t, a, st);
 }
@@ -361,7 +380,10 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
         s.follows = 1;
         TRY(launched(launch_keys(k.type, s, plan.prefix, aligned, st), "prefix attention"));
     }
-    if (plan.partial) TRY(launched(launch_paged_merge(k.type, a, plan.parts, st), "paged merge"));
+    if (a.whole >= 0)
+        TRY(launched(launch_paged_tail_merge(k.type, a, plan.own.units, st), "paged merge"));
+    else if (plan.partial && a.part_o)
+        TRY(launched(launch_paged_merge(k.type, a, plan.parts, st), "paged merge"));
     return VOX_OK;
 }
 

@@ -51,6 +51,11 @@ struct PagedAttnArgs {
     float* part_o;
     float2* part_ml;  // (maximum score in log2 units, sum)
     int part0, splits;
+    // tcgen05 kernel: the first `whole` (tile, kv head) units of the launch are not
+    // split and write `out`; where there are others behind them, they write their
+    // parts as [unit - whole][part][row of the tile] and launch_paged_tail_merge
+    // joins those.  -1: `splits` holds for all.
+    int whole;
     // 1: the launch may start before the one in front of it in the stream, an
     // attention kernel over other keys of the same call, has ended (programmatic
     // dependent launch); it reads nothing of that one and waits for it at its
@@ -61,8 +66,9 @@ struct PagedAttnArgs {
 // Upper bound on the tiles of `rows` query rows, from the host's bounds alone.
 inline int64_t paged_tiles_bound(const PagedAttnArgs& a, int rows) {
     if (a.keys_of == PagedKeysOf::PREFIX) return ((int64_t)a.n_tokens * a.group + rows - 1) / rows;
-    if ((int64_t)a.max_q * a.group <= rows) return a.n_seqs;
-    return (int64_t)a.n_tokens * a.group / rows + a.n_seqs;
+    const int64_t all = (int64_t)a.n_tokens * a.group / rows + a.n_seqs;
+    const int64_t each = (int64_t)a.n_seqs * (((int64_t)a.max_q * a.group + rows - 1) / rows);
+    return all < each ? all : each;
 }
 
 struct PagedAppendArgs {
@@ -120,6 +126,9 @@ cudaError_t launch_paged_attn_rows(PagedType t, const PagedAttnArgs& a, int nt, 
 // head_dim 64 or 128, pages of at least 8 slots, every row on a 16-byte boundary.
 cudaError_t launch_paged_attn_tiles(PagedType t, const PagedAttnArgs& a, cudaStream_t st);
 constexpr int kPagedTileRows = 256;  // query rows of a CTA
+
+// Joins the parts of the units behind the first a.whole of `units` (vox_paged_tiles.cu).
+cudaError_t launch_paged_tail_merge(PagedType t, const PagedAttnArgs& a, int units, cudaStream_t st);
 
 // Joins n_parts partial results into `out` (vox_paged.cu).
 cudaError_t launch_paged_merge(PagedType t, const PagedAttnArgs& a, int n_parts, cudaStream_t st);

@@ -276,8 +276,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t q_sm = base, ring = base + 2 * Cfg::TILE_BYTES;
 
     const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
-    const int z = blockIdx.x % a.splits, h = (blockIdx.x / a.splits) % a.n_kv;
-    const int tile = (int)(gridDim.x / a.splits / a.n_kv) - 1 - blockIdx.x / a.splits / a.n_kv;
+    // unit: (tile, kv head), the last tiles first: a sequence's later tokens see more keys
+    int z, unit, splits = a.splits, units;
+    if (a.whole < 0) {
+        unit = blockIdx.x / splits;
+        z = blockIdx.x - unit * splits;
+        units = gridDim.x / splits;
+    } else {
+        const int behind = (int)blockIdx.x - a.whole;
+        units = a.whole + ((int)gridDim.x - a.whole) / splits;
+        unit = behind < 0 ? blockIdx.x : a.whole + behind / splits;
+        z = behind < 0 ? 0 : behind % splits;
+        if (behind < 0) splits = 1;
+    }
+    const int h = unit % a.n_kv, tile = units / a.n_kv - 1 - unit / a.n_kv;
+    const bool to_part = a.part_o && (a.whole < 0 || unit >= a.whole);
 
     // ---- which rows and keys ----
     pdl_allow_dependents();
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const KeyBlocks kb = paged_key_blocks(pmin, pmax, ks.len, a.window, ks.sinks, 7);
     int b0 = 0, n = 0;
     if (any) {
-        paged_part(kb.total, z, a.splits, &b0, &n);
+        paged_part(kb.total, z, splits, &b0, &n);
         n -= b0;
     }
 
@@ -562,17 +575,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ok = __all_sync(~0u, ok);
         if (!ok && lane == 0) atomicOr(&sh.failed, 1);
         tmem_fence_after();
-        const int64_t at = ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head;
+        const int64_t at = a.whole < 0 ? ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head
+                                       : ((int64_t)(unit - a.whole) * splits + z) * (2 * kTile) + tid;
         const bool write = ok && tok >= 0;
-        if (a.part_o && write) a.part_ml[at] = make_float2(m, l);
+        if (to_part && write) a.part_ml[at] = make_float2(m, l);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bool odd = false;
         // The rows go through the tile's queries' memory (all products with them are
         // done), 32 floats or 64 results of a row at a time, so that a store covers
         // 128 bytes of a row; the 16-byte columns are swizzled by the row.
         const uint32_t stage = q_sm + t * Cfg::TILE_BYTES + (warp & 3) * (32 * 128);
-        const int64_t row_at = a.part_o ? at * HD : tok * a.o_ts + head * a.o_hs;
-        const int width = a.part_o ? 32 : 64;  // elements of 128 bytes
+        const int64_t row_at = to_part ? at * HD : tok * a.o_ts + head * a.o_hs;
+        const int width = to_part ? 32 : 64;  // elements of 128 bytes
         if (ok) {
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += width) {
@@ -589,14 +603,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 32; ++e) check += fabsf(__uint_as_float(o[e]));
                     odd |= !(check < __builtin_huge_valf());
-                    if (!a.part_o) {
+                    if (!to_part) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
                             o[e] = pack16<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (a.part_o || e < 4)
+                        if (to_part || e < 4)
                             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 +
                                                                                          ((((c - c0) / 8 + e) ^ (lane & 7)) << 4)),
                                          "r"(o[4 * e]), "r"(o[4 * e + 1]), "r"(o[4 * e + 2]), "r"(o[4 * e + 3])
@@ -614,7 +628,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                  : "r"(stage + r * 128 + ((e ^ (r & 7)) << 4))
                                  : "memory");
                     if (rw) {
-                        if (a.part_o)
+                        if (to_part)
                             *reinterpret_cast<uint4*>(a.part_o + ra + c0 + e * 4) = v;
                         else
                             *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ra + c0 + e * 8) = v;
@@ -632,10 +646,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const float rm = __shfl_sync(~0u, m, src), ri = __shfl_sync(~0u, inv, src);
             float acc[HD / 32];
             paged_redo_row<T, HD / 32>(a, ks, kb, kTile, b0, b0 + n, h, rt, rh, rp, rm, acc);
-            const int64_t ra = ((int64_t)(a.part0 + z) * a.n_tokens + rt) * a.n_heads + rh;
+            const int64_t ra = __shfl_sync(~0u, at, src);
 #pragma unroll
             for (int e = 0; e < HD / 32; ++e) {
-                if (a.part_o)
+                if (to_part)
                     a.part_o[ra * HD + lane + 32 * e] = acc[e];
                 else
                     static_cast<T*>(a.out)[rt * a.o_ts + rh * a.o_hs + lane + 32 * e] = from_f32<T>(acc[e] * ri);
@@ -662,6 +676,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     pdl_wait_prior_grids();  // the launch before this one ends first (PagedAttnArgs::follows)
 }
 
+// Joins the parts of a split unit; one warp per row of its tile.
+template <class T, int HD>
+__global__ void __launch_bounds__(128) paged_tail_merge_kernel(const __grid_constant__ PagedAttnArgs a, int units) {
+    constexpr int E = HD / 32;
+    const int lane = threadIdx.x & 31, per = 2 * kTile / 4;
+    const int behind = blockIdx.x / per, unit = a.whole + behind, r = (blockIdx.x - behind * per) * 4 + (threadIdx.x >> 5);
+    const int h = unit % a.n_kv, tile = units / a.n_kv - 1 - unit / a.n_kv;
+    int place, tok = -1, head = 0;
+    const int s = paged_find_tile(a, tile, 2 * kTile, &place);
+    if (s >= 0) {
+        const PagedSeq q = paged_seq(a, s);
+        const int row = place * (2 * kTile) + r;
+        if (row < q.nq * a.group) {
+            tok = q.q0 + row / a.group;
+            head = h * a.group + row % a.group;
+        }
+    }
+    pdl_wait_prior_grids();
+    if (tok < 0) return;
+    const int64_t at = (int64_t)behind * a.splits * (2 * kTile) + r;
+    float top = kNegInf;
+    for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_ml[at + z * (2 * kTile)].x);
+    const float base = top == kNegInf ? 0.f : top;
+    float total = 0.f, acc[E] = {};
+#pragma unroll 4
+    for (int z = 0; z < a.splits; ++z) {
+        const float2 ml = a.part_ml[at + z * (2 * kTile)];
+        const float f = ml.y == 0.f ? 0.f : fast_exp2(ml.x - base);
+        if (ml.y == 0.f) continue;
+        total = fmaf(f, ml.y, total);
+        const float* o = a.part_o + (at + z * (2 * kTile)) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, o[e], acc[e]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    T* out = static_cast<T*>(a.out) + tok * a.o_ts + head * a.o_hs + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = from_f32<T>(acc[e] * inv);
+}
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -684,7 +738,8 @@ cudaError_t launch_tiles(const PagedAttnArgs& a, const TileMaps& maps, cudaStrea
     static PagedKernelSetup setup;
     cudaError_t e = setup(reinterpret_cast<const void*>(k), TilesCfg<HD>::SMEM, false);
     if (e != cudaSuccess) return e;
-    const int64_t grid = paged_tiles_bound(a, 2 * kTile) * a.n_kv * a.splits;
+    const int64_t units = paged_tiles_bound(a, 2 * kTile) * a.n_kv;
+    const int64_t grid = a.whole < 0 ? units * a.splits : a.whole + (units - a.whole) * a.splits;
     if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
@@ -718,6 +773,25 @@ cudaError_t launch_paged_attn_tiles(PagedType t, const PagedAttnArgs& a, cudaStr
     if (t == PagedType::F16)
         return a.hd == 128 ? launch_tiles<__half, 128>(a, maps, st) : launch_tiles<__half, 64>(a, maps, st);
     return a.hd == 128 ? launch_tiles<__nv_bfloat16, 128>(a, maps, st) : launch_tiles<__nv_bfloat16, 64>(a, maps, st);
+}
+
+cudaError_t launch_paged_tail_merge(PagedType t, const PagedAttnArgs& a, int units, cudaStream_t st) {
+    const int64_t grid = (int64_t)(units - a.whole) * (2 * kTile / 4);
+    if (grid > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (t == PagedType::F16)
+        return a.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_tail_merge_kernel<__half, 128>, a, units)
+                           : cudaLaunchKernelEx(&cfg, paged_tail_merge_kernel<__half, 64>, a, units);
+    return a.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_tail_merge_kernel<__nv_bfloat16, 128>, a, units)
+                       : cudaLaunchKernelEx(&cfg, paged_tail_merge_kernel<__nv_bfloat16, 64>, a, units);
 }
 
 }  // namespace vox
