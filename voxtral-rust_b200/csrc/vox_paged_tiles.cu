@@ -30,8 +30,8 @@
 // Measured: 3200 to 3400 cycles per block of 128 keys and pair of tiles, of which
 // a softmax step's exponentials are 590 alone and 1040 beside the other tile's;
 // 9000 cycles before a CTA's first scores and 5000 after its last products.  Two
-// 2048-token chunks over 24 k and 32 k tokens (window 8192, 551 GFLOP) 533 us, 1.03
-// PFLOP/s; six prompts of 300 to 2500 tokens (151 GFLOP) 204 us.
+// 2048-token chunks over 24 k and 32 k tokens (window 8192, 551 GFLOP) 487 us, 1.13
+// PFLOP/s; six prompts of 300 to 2500 tokens (151 GFLOP) 202 us.
 //
 // Measured and not kept: 1 to 3 of 8 pairs of exponentials as polynomials on the
 // FMA pipe (2 % faster to 5 % slower at D = 64, up to 8 % slower at 128); one score
