@@ -234,6 +234,19 @@ def test_a_last_wave_of_few_tiles(V, dtype, dim, window, sinks, longest):
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
     ok = np.isfinite(want)
     assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+    # the same plan for queries that are not on 16-byte boundaries
+    odd = torch.empty(c.q.numel() + 1, device="cuda", dtype=c.q.dtype)[1:].view(c.q.shape)
+    odd.copy_(c.q)
+    got = c.run(q=odd).float().cpu().numpy()[:sum(q_len)]
+    assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+
+
+def test_windows_beyond_every_length(V):
+    for dtype, q_len in (("bf16", (1, 40)), ("f32", (3, 1))):
+        c = Case(V, torch, dtype, 8, 2, 64, 16, q_len, (90, 70), seed=29)
+        for window in (91, 1 << 31, (1 << 64) - 1):
+            got = V.paged_attention(c.cache, c.batch, c.q, sliding_window=window, n_sinks=(1 << 64) - 1)
+            c.check(got)
 
 
 @pytest.mark.parametrize("layout", ["heads", "slots", "pair"])
