@@ -1,0 +1,101 @@
+"""GPU tests of the paged-cache attention where single keys outweigh all others,
+where calls share what they should not, and where arguments are at their limits."""
+import math
+
+import numpy as np
+import pytest
+
+from tests.paged_testlib import Case
+from tests.vox_testlib import vox
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def V():
+    return vox()
+
+
+def store(c):
+    """Puts a case's changed keys and values (c.k, c.v, c.pk, c.pv) into its pool."""
+    for s in range(c.n):
+        t = np.arange(c.kv_len[s])
+        page = torch.from_numpy(c.table[s, t // c.page].astype(np.int64))
+        for pool, x in ((c.kp, c.k[s]), (c.vp, c.v[s])):
+            pool[page.cuda(), :, torch.from_numpy(t % c.page).cuda()] = x.cuda()
+    t = np.arange(c.prefix)
+    page = torch.from_numpy(c.pre[t // c.page].astype(np.int64))
+    for pool, x in ((c.kp, c.pk), (c.vp, c.pv)):
+        pool[page.cuda(), :, torch.from_numpy(t % c.page).cuda()] = x.cuda()
+
+
+def dominated(V, dtype, gap, spread, sinks, **kw):
+    """Every query scores about `gap` nats more on the keys `sinks` (of the prefix
+    where there is one) than on any other, and their values are 0: a result is what
+    the others add.  `spread` scales the others' keys; their values are positive."""
+    c = Case(V, torch, dtype, poison=False, **kw)
+    q = c.q_host
+    q[..., 0] = 8.0
+    q[..., 1:] *= 0.5
+    c.q = q.cuda()
+    for k, v in [(c.pk, c.pv)] + list(zip(c.k, c.v)):
+        k *= spread
+        k[..., 0] = 0.0
+        v.abs_()
+    k, v = (c.pk, c.pv) if c.prefix else (c.k[0], c.v[0])
+    for j in sinks:
+        k[j] = 0.0
+        k[j, :, 0] = gap * math.sqrt(c.dim) / 8.0
+        v[j] = 0.0
+    store(c)
+    return c
+
+
+def check_dominated(c, got):
+    """Beyond Case.expected's tolerance: a result below f16's normal range is
+    rounded by up to 2^-25, and the weights of the keys beside a dominating one may
+    be rounded by up to 2^-33 of that one's each, 64 of them at most in a step of
+    keys that share a scale (2^-40 of 8192 keys come to less): 2^-27 of a value."""
+    want, tol = c.expected()
+    got = got.detach().cpu().double().numpy()
+    n = sum(c.q_len)
+    top = max(float(x.float().abs().max()) for x in c.v + ([c.pv] if c.prefix else []) if x.numel())
+    if c.dtype == "f16":
+        tol = tol + 2.0 ** -25 + 2.0 ** -27 * top
+    off = np.abs(got - want)[:n] - tol[:n]
+    assert np.all(off <= 0), f"{off.max():.3e} over the tolerance; relative {np.max(np.abs(got / want - 1)[:n]):.3e}"
+
+
+DOMINATED = [
+    # heads, kv, dim, q_len, kv_len, prefix, sinks
+    (4, 1, 128, (1,), (8192,), 0, (0,)),                    # one stream's decode
+    (8, 2, 64, (1, 2, 1), (6000, 40, 700), 0, (0, 3)),      # few rows
+    (4, 1, 128, (20,), (5000,), 0, (0,)),                   # tcgen05 tiles
+    (4, 1, 64, (40, 3), (4000, 70), 0, (1500, 0)),          # the same, the dominating key in the middle too
+    (8, 2, 128, (1,) * 12, (30,) * 12, 4000, (0,)),         # a shared prefix, joined with the sequences' own
+    (4, 1, 64, (20,), (40,), 0, (1,)),                      # few keys
+]
+
+
+@pytest.mark.parametrize("dtype,gap", [("f16", 10.0), ("f16", 14.0), ("f16", 18.0), ("bf16", 16.0), ("f32", 16.0)])
+@pytest.mark.parametrize("spread", [0.0, 1.0])
+@pytest.mark.parametrize("heads,kv,dim,q_len,kv_len,prefix,sinks", DOMINATED)
+def test_keys_beside_a_dominating_one(V, dtype, spread, gap, heads, kv, dim, q_len, kv_len, prefix, sinks):
+    c = dominated(V, dtype, gap, spread, sinks, heads=heads, kv_heads=kv, dim=dim, q_len=q_len, kv_len=kv_len,
+                  prefix=prefix, seed=31)
+    check_dominated(c, c.run())
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("q_len", [(1,), (20,)])
+def test_dominating_keys_on_several_levels(V, q_len):
+    """Scores that rise and fall by up to 55 nats every few hundred keys: the
+    results follow the highest level whatever came before it, and what adds to them
+    at one level is not lost beside a key of value 0 at a higher one."""
+    c = dominated(V, "f16", 15.0, 1.0, (0, 64, 2000, 2001), heads=4, kv_heads=1, dim=128, q_len=q_len, kv_len=(4000,),
+                  seed=32)
+    for a, b, level in ((300, 700, -40.0), (1000, 1100, 3.0), (2500, 3000, -20.0)):
+        c.k[0][a:b, :, 0] = level * math.sqrt(c.dim) / 8.0
+    store(c)
+    check_dominated(c, c.run())

@@ -49,7 +49,7 @@ struct PagedAttnArgs {
     // partial results (part_o null: the kernel writes `out`).  This launch
     // writes the parts part0 .. part0 + splits - 1 of [part][token][head].
     float* part_o;
-    float2* part_ml;  // (maximum score in log2 units, sum)
+    float2* part_ml;  // (what weights are taken relative to, in log2 units; their sum)
     int part0, splits;
     // tcgen05 kernel: the first `whole` (tile, kv head) units of the launch are not
     // split and write `out`; where there are others behind them, they write their

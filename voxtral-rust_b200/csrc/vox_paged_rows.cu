@@ -14,8 +14,11 @@
 //
 // tcgen05 has no use here: its smallest tile has 64 rows.  f16 and bf16 take
 // mma.m16n8k16 with the weights rounded to the type (half a step of 2^-11 or
-// 2^-8, the size of the result's own rounding); f32 takes mma.m16n8k8 on tf32
-// halves, x = hi + lo with hi rounded to 11 bits: hi hi + hi lo + lo hi drops lo
+// 2^-8, the size of the result's own rounding; the sums are not rounded).  bf16 has
+// the exponents of f32; f16 weights are taken as 2^15 times what they are beside the
+// maximum, so that they keep all their bits down to 2^-29 of it (18 nats below a key
+// of value 0: without, these were lost) and are off by at most 2^-40 below.  f32 takes
+// mma.m16n8k8 on tf32 halves, x = hi + lo with hi rounded to 11 bits: hi hi + hi lo + lo hi drops lo
 // lo, 2^-22 of the product.  The tensor core cuts its f32 sums
 // instead of rounding them, so f32 sums over the keys are kept outside it: with
 // them inside, results over 2400 keys were 1.7e-6 off instead of 4.7e-7.
@@ -56,6 +59,7 @@ struct RowsCfg {
     static constexpr int UNITS = F32 ? (HD == 128 ? 2 : 4) : (HD == 128 ? (NT == 1 ? 4 : 6) : 8);
     static constexpr int RING = WARPS * UNITS * UNIT;
     static constexpr int OS = HD + 4;  // row stride of the partial results
+    static constexpr float TOP = std::is_same<T, __half>::value ? 15.f : 0.f;  // log2 of the weight at the maximum
     static constexpr int QF = F32 ? HD / 8 * NT * 512 : HD / 32 * NT * 512;
     static constexpr int BODY = RING > WARPS * ROWS * OS * 4 ? RING : WARPS * ROWS * OS * 4;
     static constexpr int SMEM = BODY + QF;
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const float base = m[n][x & 1] == kNegInf ? 0.f : m[n][x & 1];
+                const float base = m[n][x & 1] == kNegInf ? 0.f : m[n][x & 1] - Cfg::TOP;
                 s[n][x] = fast_exp2(s[n][x] - base);
                 l[n][x & 1] += s[n][x];
             }
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             l[n][e] += __shfl_xor_sync(~0u, l[n][e], 4);
             l[n][e] += __shfl_xor_sync(~0u, l[n][e], 8);
             l[n][e] += __shfl_xor_sync(~0u, l[n][e], 16);
-            if (g == 0) m_s[warp][n * 8 + 2 * t + e] = m[n][e], l_s[warp][n * 8 + 2 * t + e] = l[n][e];
+            if (g == 0) m_s[warp][n * 8 + 2 * t + e] = m[n][e] - Cfg::TOP, l_s[warp][n * 8 + 2 * t + e] = l[n][e];
         }
     __syncthreads();  // every warp's ring is used up
 #pragma unroll

@@ -37,11 +37,19 @@
 // FMA pipe (2 % faster to 5 % slower at D = 64, up to 8 % slower at 128); one score
 // buffer of 128 keys that both tiles use in turn (5 % slower).
 //
-// The running maximum of a row moves only when 64 new weights add up to more
-// than 2^8: until then each is at most 2^8 (f16 holds 2^15), sums are f32, and O
-// needs no rescaling; the final division by the sum takes any such factor out
-// again.  So a step of the common kind costs one FMA, one exponential, one
-// addition and half a conversion per score, and looks for no maximum.
+// A row's weights are 2^(score - m).  Its reference m, the running maximum once,
+// moves up only when 64 new weights add up to more than 2^8: until then each is at
+// most 2^8, sums are f32, and O needs no rescaling; the final division by the sum
+// takes any such factor out again.  So a step of the common kind costs one FMA, one
+// exponential, one addition and half a conversion per score, and looks for no
+// maximum.  Weights are rounded to the tensors' type (the sums are not): half a
+// step of 2^-8 or 2^-11 of each.  bf16 has the exponents of f32.  f16 has not: below
+// 2^-14 its steps stay 2^-24, so there m is the maximum less 2^8, weights add up to at
+// most 65504, and where a step's add up to less than 2^-4 (keys far below one with
+// nearly all of the weight, whose own value may be 0) m moves down to that step's
+// maximum.  What is still rounded more coarsely is a key beside one that is over 2^22
+// times its weight in the same 64: by up to 2^-33 of that one's.  (The long chunk
+// takes 503 us in a CUDA graph, 497 without the step down, which loses 18 nats.)
 #include <cuda.h>
 
 #include <type_traits>
@@ -56,7 +64,13 @@ namespace {
 constexpr int kTile = 128;  // query rows of a tile, keys of a block
 constexpr int kTileThreads = 352;
 constexpr int kStep = 64;         // keys of a softmax step
-constexpr float kRise = 256.f;    // a step's weights add up to at most this, or the maximum moves
+// Log2 of the weight at a row's maximum when the reference is set by it, and the
+// sums of a step's weights above and (f16) below which the reference moves.
+template <class T>
+struct TilesRange {
+    static constexpr bool F16 = std::is_same<T, __half>::value;
+    static constexpr float TOP = F16 ? 8.f : 0.f, RISE = F16 ? 65504.f : 256.f, FALL = 0x1p-4f;
+};
 constexpr uint32_t kTmemO = 0, kTmemS = 256, kTmemCols = 512;  // S_t buffer b at kTmemS + (2 t + b) 64
 
 template <int HD>
@@ -270,6 +284,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     using Cfg = TilesCfg<HD>;
     constexpr int U = Cfg::UNITS;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    using Range = TilesRange<T>;
     extern __shared__ unsigned char smem_raw[];
     __shared__ TilesShared sh;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -534,16 +549,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                              (a.window == 0 || j0 > pmax - a.window || j0 + kStep <= ks.sinks);
             tmem_ld64(buf, s);
             if (!all) tiles_mask(s, p - j0, ks.len - j0, a.window, ks.sinks - j0);
-            // The weights are taken with the maximum so far.  Only where their sum says
-            // that a score may have risen far above it (the first steps, mostly) is the
-            // new maximum looked for and the weights taken again.
+            // The weights are taken with the reference so far.  Only where their sum says
+            // that a score may have risen far above it (the first steps, mostly), or for
+            // f16 that all are far below it, is the maximum looked for and the weights
+            // taken again.  (Weights of less than 2^-80 of the sum so far stay as they are:
+            // the sums' range is f32's.)
             float l_new = 0.f;
             if (k > 0) l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
-            if (k == 0 || __any_sync(~0u, l_new > kRise || m == kNegInf)) {
+            const bool fell = Range::F16 && l_new < Range::FALL && l_new * 0x1p80f > l;
+            if (k == 0 || __any_sync(~0u, l_new > Range::RISE || m == kNegInf || fell)) {
                 float mx = kNegInf;
 #pragma unroll
                 for (int c = 0; c < kStep; c += 2) mx = max3(mx, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                const float m_new = fmaxf(m, mx * a.scale_log2);
+                const float want = mx * a.scale_log2 - Range::TOP, m_new = fell ? want : fmaxf(m, want);
                 const float f = m_new == kNegInf ? 1.f : fast_exp2(m - m_new);
                 m = m_new;
                 l *= f;
