@@ -99,3 +99,37 @@ def test_dominating_keys_on_several_levels(V, q_len):
         c.k[0][a:b, :, 0] = level * math.sqrt(c.dim) / 8.0
     store(c)
     check_dominated(c, c.run())
+
+
+EXPIRED = [
+    # dtype, heads, kv, dim, page, q_len, kv_len, prefix
+    ("bf16", 8, 2, 128, 16, (40,), (1500,), 0),        # the ring of K and V tiles goes round; keys end inside a page
+    ("f16", 4, 1, 64, 64, (70, 9), (900, 70), 0),      # two tiles of a sequence, one with a single row group
+    ("bf16", 8, 1, 128, 128, (20, 300), (100, 300), 0),
+    ("f16", 8, 2, 128, 16, (1,) * 40, (5,) * 40, 4000),  # parts of a prefix, then the merge
+]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,page,q_len,kv_len,prefix", EXPIRED)
+def test_expired_waits_are_reported(V, dtype, heads, kv, dim, page, q_len, kv_len, prefix):
+    """Waits that give up after a few polls while all arrives, and waits for tiles
+    that never come: the call ends, says so, and the next one is right."""
+    c = Case(V, torch, dtype, heads, kv, dim, page, q_len, kv_len, prefix=prefix, seed=33)
+    want = c.run()
+    limit = V.lib().vox_paged_test_waits
+    limit.restype = None
+    try:
+        for polls, units in ((1, -1), (2, -1), (5, -1), (1, 0), (20, 1), (20, 2), (20, 5)):
+            limit(polls, units)
+            for _ in range(3):
+                c.status.zero_()
+                out = c.run()
+                torch.cuda.synchronize()
+                # (every case has CTAs with 4 blocks of keys or more, or with one: 2 tiles)
+                assert int(c.status) in ((V.PAGED_TIMEOUT,) if units in (0, 1) else (0, V.PAGED_TIMEOUT))
+                if int(c.status) == 0:
+                    assert torch.equal(out, want)
+    finally:
+        limit(-1, -1)
+    c.status.zero_()
+    assert torch.equal(c.run(), want) and int(c.status) == 0

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
 
@@ -69,6 +70,8 @@ struct Checked {
 };
 
 constexpr size_t kMaxCount = INT32_MAX / 4;  // tokens, sequences, pages
+
+std::atomic<int> wait_polls{kPagedWaitPolls}, copy_units{INT32_MAX};
 
 int check_cache(const vox_paged_cache* c, Checked* out) {
     if (!c) return report_errorf(VOX_ERR_INVALID_ARG, "null cache");
@@ -349,6 +352,8 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
     a.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
     a.window = window >= kMaxCount * 2 ? 0 : (int)window;
     a.sinks = (int)std::min(sinks, kMaxCount * 2);
+    a.wait_polls = wait_polls.load(std::memory_order_relaxed);
+    a.copy_units = copy_units.load(std::memory_order_relaxed);
     if (p) {
         a.pfx_pages = p->pages;
         a.pfx_len = p->len;
@@ -388,6 +393,15 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
 }
 
 }  // namespace
+
+// For tests of VOX_PAGED_TIMEOUT (not part of the API), from the next call of this
+// process on: how many polls a wait of the tcgen05 kernel takes before it gives up,
+// and after how many K and V tiles a CTA stops asking for more, so that the products
+// wait in vain.  Less than 0 puts the default back.
+extern "C" void vox_paged_test_waits(int polls, int units) {
+    wait_polls.store(polls < 0 ? kPagedWaitPolls : polls, std::memory_order_relaxed);
+    copy_units.store(units < 0 ? INT32_MAX : units, std::memory_order_relaxed);
+}
 
 extern "C" int vox_paged_append_rope(const vox_paged_cache* c, const vox_paged_batch* b, const vox_rows* k_new,
                                      const vox_rows* v_new, float theta, size_t n_heads, const vox_rows* q,

@@ -61,7 +61,11 @@ struct PagedAttnArgs {
     // dependent launch); it reads nothing of that one and waits for it at its
     // end, so that whatever waits for this launch has waited for both.
     int follows;
+    // tcgen05 kernel: polls after which a wait gives up (seconds, by default), and K and
+    // V tiles that a CTA asks for at most (all, outside tests of the first)
+    int wait_polls, copy_units;
 };
+constexpr int kPagedWaitPolls = 1 << 22;
 
 // Upper bound on the tiles of `rows` query rows, from the host's bounds alone.
 inline int64_t paged_tiles_bound(const PagedAttnArgs& a, int rows) {

@@ -146,15 +146,15 @@ __device__ __forceinline__ void umma_commit_if(uint32_t leader, uint64_t* bar) {
         : "memory");
 }
 // Waits are bounded by their number of polls (each up to the hardware's own
-// suspension of a few microseconds): no clock is read on the way.
-__device__ __forceinline__ bool tiles_wait(uint64_t* bar, uint32_t parity) {
+// suspension of a few microseconds): no clock is read on the way.  The first poll
+// comes before the limit is looked at (2 % of the long chunk).
+__device__ __forceinline__ bool tiles_wait(uint64_t* bar, uint32_t parity, int polls) {
+    if (mbar_try_wait(bar, parity)) return true;
 #pragma unroll 1
-    for (int i = 0; i < (1 << 22); ++i)
+    for (int i = 1; i < polls; ++i)
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
-// A bounded wait of a whole warp, with one answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tiles_wait(bar, parity)); }
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
                                               uint64_t* bar) {
@@ -272,7 +272,7 @@ __device__ __forceinline__ float tiles_weights(const uint32_t* s, uint32_t* w, f
 }
 
 struct TilesShared {
-    uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2][2], p_full[2][2], pv_done[2][2], tail;
+    uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2][2], p_full[2][2], pv_done[2][2], tail, drained[2];
     uint32_t tmem;
     int lo[8], hi[8];  // smallest and largest index of a warp's rows
     int failed;
@@ -388,6 +388,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mbar_init(&sh.pv_done[t][b], 1);
             }
         mbar_init(&sh.tail, 1);
+        mbar_init(&sh.drained[0], 1);
+        mbar_init(&sh.drained[1], 1);
         fence_barrier_init();
     }
     tmem_fence_before();
@@ -410,16 +412,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         n -= b0;
     }
 
+    // Bounded waits: of a thread, and of a whole warp with one answer.
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return tiles_wait(bar, parity, a.wait_polls); };
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, wait(bar, parity)); };
     if (warp == 10) {
         // ---- K and V tiles ----
         const int ps = 1 << a.page_shift;
         const int box = min(ps, kTile), boxes = kTile / box;
         bool ok = true;
+        const int units = min(2 * n, a.copy_units);
         int issued = 0;
-        for (int i = 0; i < 2 * n && ok; ++i) {
+        for (int i = 0; i < units && ok; ++i) {
             const int slot = i % U, blk = kb.block(b0 + (i >> 1));
-            if (i >= U) ok = tiles_wait(&sh.kv_empty[slot], (i / U - 1) & 1);
-            ok = __all_sync(~0u, ok);
+            if (i >= U) ok = warp_wait(&sh.kv_empty[slot], (i / U - 1) & 1);
             if (!ok) break;
             const int j0 = blk * kTile;
             // a page that ends the keys: what lies behind them in it must not reach P V
@@ -443,8 +448,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
             issued = i + 1;
             if (ragged) {
-                ok = __all_sync(~0u, tiles_wait(&sh.tail, 0));
-                if (!ok) break;
+                ok = warp_wait(&sh.tail, 0);
+                if (!ok) {
+                    tiles_wait(&sh.tail, 0, kPagedWaitPolls);
+                    issued = i;
+                    break;
+                }
                 const int r0 = kb.end - j0, r1 = (r0 + box - 1) & ~(box - 1);
                 for (int e = lane; e < (r1 - r0) * (HD / 8); e += 32) {
                     const int r = r0 + e / (HD / 8), c = e % (HD / 8);
@@ -458,11 +467,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (lane == 0) mbar_arrive(&sh.kv_full[slot]);
             }
         }
-        if (!ok) {
-            // nothing may still be on its way into this CTA's memory when it ends
-            if (lane == 0) atomicOr(&sh.failed, 1);
-            for (int i = max(0, issued - U); i < issued; ++i) tiles_wait(&sh.kv_full[i % U], (i / U) & 1);
-        }
+        if (!ok && lane == 0) atomicOr(&sh.failed, 1);
+        // Nothing may still be on its way into this CTA's memory when it ends, whichever
+        // wait it was that expired (a unit that `tail` stood for has been waited for).
+        for (int i = max(0, issued - U); i < issued; ++i) tiles_wait(&sh.kv_full[i % U], (i / U) & 1, kPagedWaitPolls);
     } else if (warp >= 8) {
         // ---- products of tile t ----
         const int t = warp - 8, steps = t == 0 || two ? n : 0;
@@ -518,6 +526,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             free_unit(2 * i + 2);
         }
         if (!ok && steps > 0 && lane == 0) atomicOr(&sh.failed, 1);
+        // No product may be in flight when its memory goes, whichever wait expired: the
+        // thread that issued them commits them.
+        umma_commit_if(leader, &sh.drained[t]);
+        tiles_wait(&sh.drained[t], 0, kPagedWaitPolls);
     } else {
         // ---- softmax ----
         const int t = warp >> 2;
@@ -539,7 +551,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int steps = t == 0 || two ? 2 * n : 0;
 #pragma unroll 1
         for (int k = 0; k < steps; ++k) {
-            ok = __all_sync(~0u, tiles_wait(&sh.s_full[t][k & 1], (k >> 1) & 1));
+            ok = warp_wait(&sh.s_full[t][k & 1], (k >> 1) & 1);
             if (!ok) break;
             tmem_fence_after();
             const uint32_t buf = t_s + (k & 1) * kStep;
@@ -566,7 +578,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 m = m_new;
                 l *= f;
                 if (k > 0) {
-                    ok = __all_sync(~0u, tiles_wait(&sh.pv_done[t][(k - 1) & 1], ((k - 1) >> 1) & 1));
+                    ok = warp_wait(&sh.pv_done[t][(k - 1) & 1], ((k - 1) >> 1) & 1);
                     if (!ok) break;
                     tmem_fence_after();
 #pragma unroll 1
@@ -589,8 +601,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (lane == 0) mbar_arrive(&sh.p_full[t][k & 1]);
         }
         // ---- the result ----
-        if (ok && steps > 0) ok = tiles_wait(&sh.pv_done[t][1], (n - 1) & 1);
-        ok = __all_sync(~0u, ok);
+        if (ok && steps > 0) ok = warp_wait(&sh.pv_done[t][1], (n - 1) & 1);
         if (!ok && lane == 0) atomicOr(&sh.failed, 1);
         tmem_fence_after();
         const int64_t at = a.whole < 0 ? ((int64_t)(a.part0 + z) * a.n_tokens + tok) * a.n_heads + head
@@ -676,17 +687,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_fence_before();
     }
     __syncthreads();
-    if (sh.failed) {
-        // products may be in flight: let them end before their memory goes
-        if (warp >= 8 && warp < 10 && lane == 0) {
-            paged_status(a, VOX_PAGED_TIMEOUT);
-            mbar_init(&sh.q_full[warp - 8], 1);
-            fence_barrier_init();
-            umma_commit(&sh.q_full[warp - 8]);
-            tiles_wait(&sh.q_full[warp - 8], 0);
-        }
-        __syncthreads();
-    }
+    if (tid == 0 && sh.failed) paged_status(a, VOX_PAGED_TIMEOUT);
     if (warp == 8) {
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
