@@ -570,8 +570,8 @@ int vox_attention_gqa_step_noalloc(const float* d_query, const float* d_keys,
  * the calls are asynchronous on `stream` (a cudaStream_t, 0 = default
  * stream), allocate nothing, keep nothing between calls, may be captured into
  * a graph, and leave the calling thread's current device as it was.  A CUDA
- * error already pending on the calling thread is reported as VOX_ERR_CUDA and
- * nothing is launched.  (What a call keeps is that a kernel's limits have been
+ * error already pending on the calling thread is reported once, as VOX_ERR_CUDA,
+ * and nothing is launched.  (What a call keeps is that a kernel's limits have been
  * raised on a device: not after cudaDeviceReset.)  All
  * tensors of a call have the cache's dtype: VOX_DT_F32, VOX_DT_F16 or
  * VOX_DT_BF16.  Strides are in elements.

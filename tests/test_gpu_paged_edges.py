@@ -133,3 +133,15 @@ def test_expired_waits_are_reported(V, dtype, heads, kv, dim, page, q_len, kv_le
         limit(-1, -1)
     c.status.zero_()
     assert torch.equal(c.run(), want) and int(c.status) == 0
+
+
+def test_a_call_after_a_failed_allocation(V):
+    """The failure is the failed call's alone."""
+    cfg = V.DecoderConfig(dim=8, hidden_dim=16, n_heads=2, n_kv_heads=1, head_dim=4, sliding_window=4, norm_eps=1e-5,
+                          rope_theta=1e4)
+    c = Case(V, torch, "bf16", 8, 2, 64, 16, (1, 2), (40, 90), seed=34)
+    with V.Context(cfg) as ctx:
+        with pytest.raises(V.VoxError) as e:
+            V.RollingKvCache(ctx, 4, 8, 128, 1 << 29)  # 8 TB and more
+        assert e.value.code == V.ERR_OOM
+        c.check(c.run())

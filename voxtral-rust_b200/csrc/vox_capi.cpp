@@ -27,6 +27,13 @@ namespace {
 
 thread_local std::string g_err;
 
+// A CUDA error that is reported is done with: left on the thread, a later call that
+// asks for the last error would take it for its own.  (One that the context does not
+// survive comes back by itself.)
+void forget_cuda_error(int code) {
+    if (code == VOX_ERR_CUDA || code == VOX_ERR_OOM) (void)cudaGetLastError();
+}
+
 int fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
@@ -34,6 +41,7 @@ int fail(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     g_err = buf;
+    forget_cuda_error(code);
     return code;
 }
 
@@ -222,7 +230,10 @@ BgChain chain_of(const BgArgs& a, const BgPlan& p) {
 
 }  // namespace
 
-int vox::report_error(int code, const char* msg) { return fail(code, "%s", msg); }
+int vox::report_error(int code, const char* msg) {
+    g_err = msg;
+    return code;
+}
 
 int vox::report_errorf(int code, const char* fmt, ...) {
     char buf[512];
@@ -231,6 +242,7 @@ int vox::report_errorf(int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
     g_err = buf;
+    forget_cuda_error(code);
     return code;
 }
 

@@ -22,6 +22,7 @@
 
 #include "../../include/vox_decoder.h"
 #include "vox_device.cuh"
+#include "vox_host.h"
 
 namespace vox {
 
@@ -70,11 +71,11 @@ int setup_device(int dev, DeviceSetup** out) {
     if (!s.ready) {
         void* p = nullptr;
         cudaError_t e = cudaGetSymbolAddress(&p, g_attn_scratch);
-        if (e != cudaSuccess) return report_error(VOX_ERR_CUDA, "cudaGetSymbolAddress(scratch) failed");
+        if (e != cudaSuccess) return report_errorf(VOX_ERR_CUDA, "cudaGetSymbolAddress(scratch) failed");
         e = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
-        if (e != cudaSuccess) return report_error(VOX_ERR_CUDA, "cannot read the SM count");
+        if (e != cudaSuccess) return report_errorf(VOX_ERR_CUDA, "cannot read the SM count");
         e = attn_prepare(dev);
-        if (e != cudaSuccess) return report_error(VOX_ERR_CUDA, "cannot set the attention smem limit");
+        if (e != cudaSuccess) return report_errorf(VOX_ERR_CUDA, "cannot set the attention smem limit");
         s.scratch = static_cast<unsigned char*>(p);
         s.ready = true;
     }
@@ -103,7 +104,7 @@ extern "C" int vox_attention_gqa_step_noalloc(const float* d_query, const float*
 
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices)
-        return report_error(VOX_ERR_CUDA, "no usable current CUDA device");
+        return report_errorf(VOX_ERR_CUDA, "no usable current CUDA device");
     DeviceSetup* s = nullptr;
     int rc = setup_device(dev, &s);
     if (rc != VOX_OK) return rc;

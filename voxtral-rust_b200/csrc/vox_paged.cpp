@@ -26,9 +26,12 @@ namespace {
 class DeviceGuard {
   public:
     int enter(int device) {
-        // An error left by earlier work is the caller's: reported, not mistaken for one of this call.
-        if (cudaPeekAtLastError() != cudaSuccess)
-            return report_errorf(VOX_ERR_CUDA, "an earlier CUDA error is pending on this thread; nothing was launched");
+        // An error left by earlier work: reported once, not mistaken for one of this call.
+        // (Without a driver every call of the runtime answers so.)
+        const cudaError_t earlier = cudaGetLastError();
+        if (earlier != cudaSuccess && earlier != cudaErrorInsufficientDriver && earlier != cudaErrorNoDevice)
+            return report_errorf(VOX_ERR_CUDA, "an earlier CUDA error was pending on this thread (%s); nothing was launched",
+                                 cudaGetErrorString(earlier));
         if (cudaGetDevice(&before_) != cudaSuccess) return no_device(device);
         if (before_ != device) {
             if (cudaSetDevice(device) != cudaSuccess) return no_device(device);
