@@ -616,7 +616,8 @@ typedef struct vox_paged_batch {
 #define VOX_PAGED_BAD_LENGTH 1u
 #define VOX_PAGED_BAD_PAGE 2u
 #define VOX_PAGED_TIMEOUT 4u /* a bounded wait inside a kernel expired: the outputs are incomplete */
-/* [n_tokens, heads, head_dim] with a unit last stride; both strides 0 = packed. */
+/* [n_tokens, heads, head_dim] with a unit last stride; both strides 0 = packed.
+ * Rows that a call writes must not overlap; those it reads may. */
 typedef struct vox_rows {
     void* ptr;
     size_t token_stride, head_stride;
@@ -624,8 +625,10 @@ typedef struct vox_rows {
 /* Keys and values of the batch's tokens into their slots, the keys rotated as
  * vox_rope_interleaved_inplace does at position first_pos + index (angles
  * exact modulo a turn at any position), and, where q is not NULL, the queries
- * rotated from q to q_out (which may be q itself).  rope_theta 0: no rotation;
- * otherwise >= 1.  A token before the cache's first slot (kv_len < q_len) is
+ * rotated from q to q_out (which may be q itself, with the same strides, and
+ * must not overlap it otherwise).  The rows of the pool, and of q_out, must not
+ * overlap one another: strides that do not keep them apart, one inside the next,
+ * are refused.  rope_theta 0: no rotation; otherwise >= 1.  A token before the cache's first slot (kv_len < q_len) is
  * not stored.  Two tokens of a call must not have the same slot. */
 int vox_paged_append_rope(const vox_paged_cache* cache, const vox_paged_batch* batch, const vox_rows* k_new,
                           const vox_rows* v_new, float rope_theta, size_t n_heads, const vox_rows* q,

@@ -24,3 +24,41 @@ def test_an_error_that_was_reported_is_not_reported_again(V):
         assert e.value.code == V.ERR_CUDA
         assert V.lib().vox_paged_append_rope(c, b, r, r, 1e4, 4, r, r, None) == V.ERR_CUDA
         assert "cannot use device" in V.last_error()
+
+
+def test_rows_that_are_written_must_not_overlap(V):
+    """3 tokens of 4 heads of 64."""
+    L = V.lib()
+    c, b, _, r = (C.byref(x) for x in descs(V))
+    for token, head in ((64, 64), (255, 64), (64, 191), (256, 63), (100, 100)):
+        out = C.byref(descs(V, rows=dict(ptr=OUT, token_stride=token, head_stride=head))[3])
+        refused(V, L.vox_paged_attention(c, b, r, 4, 0, 0, 0.0, out, None, 0, None), "ERR_SHAPE", "strides")
+        refused(V, L.vox_paged_append_rope(c, b, r, r, 1e4, 4, r, out, None), "ERR_SHAPE", "strides")
+    for token, head in ((256, 64), (64, 192), (1000, 100), (1 << 40, 64)):
+        out = C.byref(descs(V, rows=dict(ptr=OUT, token_stride=token, head_stride=head))[3])
+        if not cuda_available():  # (made-up addresses: past the checks there is only the missing device)
+            assert L.vox_paged_attention(c, b, r, 4, 0, 0, 0.0, out, None, 0, None) == V.ERR_CUDA
+            assert L.vox_paged_append_rope(c, b, r, r, 1e4, 4, r, out, None) == V.ERR_CUDA
+
+
+def test_a_pool_that_is_written_must_not_overlap(V):
+    """10 pages of 2 heads of 16 slots of 64."""
+    L = V.lib()
+    for page, head, slot in ((64, 64, 64), (2047, 1024, 64), (2048, 64, 64), (2048, 1023, 64), (2048, 64, 127),
+                             (1024, 1024, 64), (64, 640, 640)):
+        c, b, _, r = (C.byref(x) for x in descs(V, cache=dict(page_stride=page, head_stride=head, slot_stride=slot)))
+        refused(V, L.vox_paged_append_rope(c, b, r, r, 1e4, 4, r, r, None), "ERR_SHAPE", "strides")
+    for page, head, slot in ((2048, 1024, 64), (2048, 64, 128), (4096, 1024, 64), (64, 10240, 640), (64, 640, 1280)):
+        c, b, _, r = (C.byref(x) for x in descs(V, cache=dict(page_stride=page, head_stride=head, slot_stride=slot)))
+        if not cuda_available():
+            assert L.vox_paged_append_rope(c, b, r, r, 1e4, 4, r, r, None) == V.ERR_CUDA
+
+
+def test_queries_in_place_keep_their_strides(V):
+    L = V.lib()
+    c, b, _, r = (C.byref(x) for x in descs(V))
+    wide = C.byref(descs(V, rows=dict(token_stride=512, head_stride=64))[3])
+    for q, out in ((r, wide), (wide, r)):
+        refused(V, L.vox_paged_append_rope(c, b, r, r, 1e4, 4, q, out, None), "ERR_SHAPE", "strides")
+    if not cuda_available():
+        assert L.vox_paged_append_rope(c, b, r, r, 1e4, 4, wide, wide, None) == V.ERR_CUDA

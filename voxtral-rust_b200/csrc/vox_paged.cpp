@@ -128,6 +128,25 @@ int check_batch(const vox_paged_cache* c, const vox_paged_batch* b) {
     return VOX_OK;
 }
 
+// Whether rows of `hd` elements at multiples of the strides are kept apart by them:
+// sorted, each stride steps over all that the smaller ones reach.
+struct Dim {
+    size_t n, stride;
+};
+bool rows_apart(std::initializer_list<Dim> dims, size_t hd) {
+    Dim d[3];
+    size_t n = 0;
+    for (const Dim& x : dims)
+        if (x.n > 1) d[n++] = x;
+    std::sort(d, d + n, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    unsigned __int128 reach = hd;
+    for (size_t i = 0; i < n; ++i) {
+        if (d[i].stride < reach) return false;
+        reach += (unsigned __int128)(d[i].n - 1) * d[i].stride;
+    }
+    return true;
+}
+
 // [n_tokens, heads, head_dim] rows: strides, alignment to the type.  Rows that
 // are written must not overlap.
 int check_rows(const vox_rows* r, const char* name, size_t tokens, size_t heads, size_t hd, PagedType t, bool written,
@@ -142,8 +161,8 @@ int check_rows(const vox_rows* r, const char* name, size_t tokens, size_t heads,
     }
     if (std::max(r->token_stride, r->head_stride) > (size_t(1) << 40))
         return report_errorf(VOX_ERR_SHAPE, "%s strides out of range", name);
-    if (written && ((tokens > 1 && r->token_stride < hd) || (heads > 1 && r->head_stride < hd)))
-        return report_errorf(VOX_ERR_SHAPE, "%s strides must be at least head_dim", name);
+    if (written && !rows_apart({{tokens, r->token_stride}, {heads, r->head_stride}}, hd))
+        return report_errorf(VOX_ERR_SHAPE, "%s strides must be at least head_dim and keep its rows apart", name);
     *ts = (int64_t)r->token_stride;
     *hs = (int64_t)r->head_stride;
     return VOX_OK;
@@ -416,6 +435,9 @@ extern "C" int vox_paged_append_rope(const vox_paged_cache* c, const vox_paged_b
         return report_errorf(VOX_ERR_INVALID_ARG, "rope_theta must be 0 or finite and >= 1");
     if (q && (n_heads == 0 || n_heads > 65536)) return report_errorf(VOX_ERR_INVALID_ARG, "n_heads must be in 1..65536");
     if (b->n_seqs == 0 || b->n_tokens == 0) return VOX_OK;
+    if (!rows_apart({{c->n_pages, (size_t)k.page_stride}, {c->n_kv_heads, (size_t)k.head_stride}, {c->page_size, (size_t)k.slot_stride}},
+                    c->head_dim))
+        return report_errorf(VOX_ERR_SHAPE, "cache strides must keep the rows of a pool that is written apart");
     PagedAppendArgs a{};
     fill_common(a, c, k, b);
     a.k = c->keys;
@@ -428,6 +450,9 @@ extern "C" int vox_paged_append_rope(const vox_paged_cache* c, const vox_paged_b
     if (q) {
         TRY(check_rows(q, "q", b->n_tokens, n_heads, c->head_dim, k.type, false, &a.q_ts, &a.q_hs));
         TRY(check_rows(q_out, "q_out", b->n_tokens, n_heads, c->head_dim, k.type, true, &a.qo_ts, &a.qo_hs));
+        // in place, every thread writes what it has read itself
+        if (q_out->ptr == q->ptr && ((b->n_tokens > 1 && a.q_ts != a.qo_ts) || (n_heads > 1 && a.q_hs != a.qo_hs)))
+            return report_errorf(VOX_ERR_SHAPE, "q_out in the place of q must have its strides");
         a.q = q->ptr;
         a.q_out = q_out->ptr;
         a.n_heads = (int)n_heads;
