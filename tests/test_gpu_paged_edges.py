@@ -145,3 +145,17 @@ def test_a_call_after_a_failed_allocation(V):
             V.RollingKvCache(ctx, 4, 8, 128, 1 << 29)  # 8 TB and more
         assert e.value.code == V.ERR_OOM
         c.check(c.run())
+
+
+def test_a_batch_serves_pools_of_different_page_sizes(V):
+    """Each call has the bound of its own pool, whatever calls another thread makes
+    with the same batch in between."""
+    c = Case(V, torch, "bf16", 8, 2, 64, 16, (1, 2), (70, 90), seed=35)
+    small = Case(V, torch, "bf16", 8, 2, 64, 8, (1,), (5,), seed=36)
+    import ctypes as C
+    mine = C.cast(c.batch._for(c.cache), C.POINTER(V.PagedBatchDesc)).contents
+    other = C.cast(c.batch._for(small.cache), C.POINTER(V.PagedBatchDesc)).contents
+    width = c.table_dev.shape[1]
+    assert (mine.max_kv_len, other.max_kv_len) == (16 * width, 8 * width)
+    c.check(c.run())
+    assert int(c.status) == 0

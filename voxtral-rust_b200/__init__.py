@@ -1231,7 +1231,7 @@ class PagedBatch:
         self.device, self.n_seqs, self.n_tokens = kv_len.device, n, int(n_tokens)
         self._keep = (q_start, kv_len, page_table, first_pos, status)
         width = int(page_table.shape[1])
-        self._auto_max_kv = max_kv_len is None
+        self._by_page_size = {} if max_kv_len is None else None
         self.desc = PagedBatchDesc(n, self.n_tokens, int(max_q_len), 0 if max_kv_len is None else int(max_kv_len),
                                    width, int(page_table.stride(0)) if n > 1 else width, q_start.data_ptr(),
                                    kv_len.data_ptr(), page_table.data_ptr(),
@@ -1243,9 +1243,16 @@ class PagedBatch:
     def _for(self, cache):
         if self.device != cache.device:
             raise ValueError("the batch and the cache must be on one device")
-        if self._auto_max_kv:
-            self.desc.max_kv_len = self.desc.table_width * cache.page_size
-        return self._ref
+        if self._by_page_size is None:
+            return self._ref
+        # a description for every page size, never changed once it is there: another
+        # thread's call may be reading it
+        desc = self._by_page_size.get(cache.page_size)
+        if desc is None:
+            desc = PagedBatchDesc.from_buffer_copy(self.desc)
+            desc.max_kv_len = desc.table_width * cache.page_size
+            desc = self._by_page_size.setdefault(cache.page_size, desc)
+        return C.addressof(desc)
 
 
 def _paged_rows(t, name, batch, heads, cache):
@@ -1293,8 +1300,7 @@ def _paged_attention(cache, batch, prefix, max_prefix, q, sliding_window, n_sink
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     orow = _paged_rows(out, "out", batch, heads, cache)
     # the scratch size follows from the host's bounds alone
-    what = (heads, sliding_window, n_sinks, max_prefix, batch.desc.max_kv_len, cache.dtype, cache.n_kv_heads,
-            cache.head_dim, cache.page_size)
+    what = (heads, sliding_window, n_sinks, max_prefix, cache.dtype, cache.n_kv_heads, cache.head_dim, cache.page_size)
     n = batch._workspace_bytes.get(what)
     if n is None:
         got = SZ()
