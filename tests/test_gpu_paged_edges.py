@@ -159,3 +159,29 @@ def test_a_batch_serves_pools_of_different_page_sizes(V):
     assert (mine.max_kv_len, other.max_kv_len) == (16 * width, 8 * width)
     c.check(c.run())
     assert int(c.status) == 0
+
+
+def test_a_batch_tells_what_its_calls_met(V):
+    """Without a status tensor of the caller's too."""
+    c = Case(V, torch, "bf16", 8, 2, 64, 16, (1, 40), (70, 90), seed=37, poison=False)
+    batch = V.PagedBatch(c.q_start, c.kv, c.table_dev, c.tokens, 40)
+    V.paged_attention(c.cache, batch, c.q)
+    batch.check()
+    c.kv[0] = -1
+    V.paged_attention(c.cache, batch, c.q)
+    with pytest.raises(V.VoxError, match="lengths") as e:
+        batch.check()
+    assert e.value.code == V.ERR_RANGE and "page ids" not in e.value.message
+    batch.check()  # cleared
+    c.kv[0] = 70
+    c.table_dev[1, 0] = c.n_pages
+    k = torch.zeros(c.tokens, 2, 64, device="cuda", dtype=torch.bfloat16)
+    c.kv[1] = 40
+    V.paged_append_rope(c.cache, batch, k, k, 0.0)
+    with pytest.raises(V.VoxError, match="page ids"):
+        batch.check()
+    mine = V.PagedBatch(c.q_start, c.kv, c.table_dev, c.tokens, 40, status=c.status)
+    V.paged_attention(c.cache, mine, c.q)
+    with pytest.raises(V.VoxError, match="page ids"):
+        mine.check()
+    assert int(c.status) == 0

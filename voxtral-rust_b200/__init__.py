@@ -1203,10 +1203,14 @@ class PagedBatch:
 
     q_start int32 [n_seqs + 1], kv_len int32 [n_seqs], page_table int32
     [n_seqs, pages], first_pos (absolute position of each sequence's index 0;
-    default 0) int64 [n_seqs] and status (VOX_PAGED_* bits) int32 [1] are CUDA
-    tensors, read when the kernels run: a captured graph follows them within
-    the host's bounds n_tokens, max_q_len and max_kv_len (default: the table's
-    capacity)."""
+    default 0) int64 [n_seqs] and status (VOX_PAGED_* bits, default: a word of
+    the batch's own) int32 [1] are CUDA tensors, read when the kernels run: a
+    captured graph follows them within the host's bounds n_tokens, max_q_len
+    and max_kv_len (default: the table's capacity).
+
+    A sequence whose lengths are out of these bounds is skipped: its rows of a
+    new output are undefined.  Calls do not wait to see that: check() does, for
+    all calls with the batch since the last one."""
 
     def __init__(self, q_start, kv_len, page_table, n_tokens, max_q_len, max_kv_len=None, first_pos=None, status=None):
         import torch
@@ -1228,7 +1232,9 @@ class PagedBatch:
                 raise ValueError("q_start, kv_len, first_pos and status must be contiguous")
         if page_table.shape[1] > 1 and page_table.stride(1) != 1:
             raise ValueError("the rows of page_table must be contiguous")
-        self.device, self.n_seqs, self.n_tokens = kv_len.device, n, int(n_tokens)
+        if status is None:
+            status = torch.zeros(1, dtype=i32, device=kv_len.device)
+        self.device, self.n_seqs, self.n_tokens, self.status = kv_len.device, n, int(n_tokens), status
         self._keep = (q_start, kv_len, page_table, first_pos, status)
         width = int(page_table.shape[1])
         self._by_page_size = {} if max_kv_len is None else None
@@ -1236,7 +1242,7 @@ class PagedBatch:
                                    width, int(page_table.stride(0)) if n > 1 else width, q_start.data_ptr(),
                                    kv_len.data_ptr(), page_table.data_ptr(),
                                    first_pos.data_ptr() if first_pos is not None else None,
-                                   status.data_ptr() if status is not None else None)
+                                   status.data_ptr())
         self._ref = C.addressof(self.desc)
         self._workspace_bytes = {}
 
@@ -1253,6 +1259,20 @@ class PagedBatch:
             desc.max_kv_len = desc.table_width * cache.page_size
             desc = self._by_page_size.setdefault(cache.page_size, desc)
         return C.addressof(desc)
+
+    def check(self):
+        """Waits for the current stream's calls with this batch and raises where
+        one of them met bad lengths, a bad page or an expired wait; clears the
+        status word."""
+        bits = int(self.status.item())
+        if not bits:
+            return
+        self.status.zero_()
+        what = [text for bit, text in ((PAGED_BAD_LENGTH, "lengths out of bounds: sequences were skipped"),
+                                       (PAGED_BAD_PAGE, "page ids outside the pool: read as zeros, not written"),
+                                       (PAGED_TIMEOUT, "a bounded wait inside a kernel expired: outputs are incomplete"))
+                if bits & bit]
+        raise VoxError(ERR_DEVICE_TIMEOUT if bits & PAGED_TIMEOUT else ERR_RANGE, "paged batch: " + "; ".join(what))
 
 
 def _paged_rows(t, name, batch, heads, cache):
@@ -1328,7 +1348,8 @@ def paged_attention(cache: PagedKvCache, batch: PagedBatch, q, sliding_window=0,
     n_heads, head_dim] over the cache: a token sees the last sliding_window
     tokens (0: all), its own included, and the first n_sinks of its sequence.
     scale 0 = 1/sqrt(head_dim).  Returns out [n_tokens, n_heads, head_dim];
-    rows behind the last sequence are left as they were (vox_paged_attention)."""
+    rows behind the last sequence, and those of a sequence that is skipped
+    (PagedBatch.check), are left as they were (vox_paged_attention)."""
     return _paged_attention(cache, batch, None, None, q, sliding_window, n_sinks, scale, out)
 
 
