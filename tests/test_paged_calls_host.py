@@ -62,3 +62,9 @@ def test_queries_in_place_keep_their_strides(V):
         refused(V, L.vox_paged_append_rope(c, b, r, r, 1e4, 4, q, out, None), "ERR_SHAPE", "strides")
     if not cuda_available():
         assert L.vox_paged_append_rope(c, b, r, r, 1e4, 4, wide, wide, None) == V.ERR_CUDA
+
+
+def test_negative_windows_and_sinks_are_refused(V):
+    for kw in (dict(sliding_window=-1), dict(n_sinks=-3)):
+        with pytest.raises(ValueError, match="sliding_window and n_sinks"):
+            V.paged_attention(None, None, None, **kw)

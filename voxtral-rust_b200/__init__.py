@@ -1312,6 +1312,8 @@ def paged_append_rope(cache: PagedKvCache, batch: PagedBatch, k_new, v_new, rope
 
 
 def _paged_attention(cache, batch, prefix, max_prefix, q, sliding_window, n_sinks, scale, out):
+    if sliding_window < 0 or n_sinks < 0:  # (a size_t would take them as far beyond every length)
+        raise ValueError("sliding_window and n_sinks must be >= 0")
     torch, stream, L = _paged_env()
     ref = batch._for(cache)
     heads = q.shape[1] if q.dim() == 3 else 0
@@ -1367,5 +1369,7 @@ def paged_prefix_attention(cache: PagedKvCache, batch: PagedBatch, prefix_pages,
     if prefix_pages.get_device() != cache.index or prefix_len.get_device() != cache.index:
         raise ValueError("the prefix and the cache must be on one device")
     max_prefix_len = int(max_prefix_len)
+    if max_prefix_len < 0:
+        raise ValueError("max_prefix_len must be >= 0")
     prefix = _pack_prefix(prefix_pages.data_ptr(), prefix_len.data_ptr(), prefix_pages.shape[0], max_prefix_len)
     return _paged_attention(cache, batch, prefix, max_prefix_len, q, sliding_window, n_sinks, scale, out)
