@@ -68,3 +68,11 @@ def test_negative_windows_and_sinks_are_refused(V):
     for kw in (dict(sliding_window=-1), dict(n_sinks=-3)):
         with pytest.raises(ValueError, match="sliding_window and n_sinks"):
             V.paged_attention(None, None, None, **kw)
+
+
+def test_scales_that_overflow_are_refused(V):
+    """The kernels work in powers of two: scale times log2(e) has to be finite."""
+    c, b, p, r = (C.byref(x) for x in descs(V))
+    L = V.lib()
+    refused(V, L.vox_paged_attention(c, b, r, 4, 0, 0, 3e38, r, None, 0, None), "ERR_INVALID_ARG", "scale")
+    refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 3e38, r, None, 0, None), "ERR_INVALID_ARG", "scale")

@@ -72,6 +72,8 @@ struct Checked {
     int page_shift;
 };
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 constexpr size_t kMaxCount = INT32_MAX / 4;  // tokens, sequences, pages
 
 std::atomic<int> wait_polls{kPagedWaitPolls}, copy_units{INT32_MAX};
@@ -358,7 +360,8 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
               void* stream) {
     Checked k;
     TRY(check_attention(c, b, p, n_heads, &k));
-    if (!(scale >= 0.f) || !std::isfinite(scale)) return report_errorf(VOX_ERR_INVALID_ARG, "scale must be finite and >= 0");
+    if (!(scale >= 0.f) || !std::isfinite(scale * kLog2e))
+        return report_errorf(VOX_ERR_INVALID_ARG, "scale must be >= 0 and, times log2(e), finite");
     if (b->n_seqs == 0 || b->n_tokens == 0) return VOX_OK;
     PagedAttnArgs a{};
     fill_common(a, c, k, b);
@@ -371,7 +374,7 @@ int attention(const vox_paged_cache* c, const vox_paged_batch* b, const vox_page
     a.out = out->ptr;
     a.n_heads = (int)n_heads;
     a.group = (int)(n_heads / c->n_kv_heads);
-    a.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
+    a.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * kLog2e;
     a.window = window >= kMaxCount * 2 ? 0 : (int)window;
     a.sinks = (int)std::min(sinks, kMaxCount * 2);
     a.wait_polls = wait_polls.load(std::memory_order_relaxed);
