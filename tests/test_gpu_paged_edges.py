@@ -185,3 +185,12 @@ def test_a_batch_tells_what_its_calls_met(V):
     with pytest.raises(V.VoxError, match="page ids"):
         mine.check()
     assert int(c.status) == 0
+
+
+def test_a_batch_that_lives_on_keeps_little(V):
+    c = Case(V, torch, "bf16", 8, 2, 64, 16, (1, 2), (70, 90), seed=38, poison=False)
+    want = V.paged_attention(c.cache, c.batch, c.q, sliding_window=1000)
+    for n in range(300):
+        got = V.paged_attention(c.cache, c.batch, c.q, sliding_window=1000 + n, n_sinks=n)
+        assert torch.equal(got, want)
+    assert len(c.batch._workspace_bytes) <= 64

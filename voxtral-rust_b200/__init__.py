@@ -1331,6 +1331,8 @@ def _paged_attention(cache, batch, prefix, max_prefix, q, sliding_window, n_sink
         else:
             _check(L.vox_paged_prefix_attention_workspace(cache._ref, ref, prefix, heads, sliding_window, n_sinks,
                                                           C.byref(got)))
+        if len(batch._workspace_bytes) >= 64:  # a batch that lives on while its bounds change
+            batch._workspace_bytes.clear()
         n = batch._workspace_bytes[what] = got.value
     ws = torch.empty(n, dtype=torch.uint8, device=cache.device) if n else None
     wp = ws.data_ptr() if n else None
