@@ -600,7 +600,9 @@ typedef struct vox_paged_cache {
  *
  * The device arrays are checked by the kernels.  A sequence whose lengths are
  * negative, out of order or beyond the bounds or its table row is skipped
- * (nothing of it is read or written) and VOX_PAGED_BAD_LENGTH set in *status;
+ * (nothing of it is read or written) and VOX_PAGED_BAD_LENGTH set in *status
+ * (where q_start does not ascend, tokens of the sequences around may be skipped
+ * with it);
  * a page id outside the pool, where a visible or new token needs it, reads as
  * zeros, is not written, and sets VOX_PAGED_BAD_PAGE.  *status (nullable)
  * receives bits by atomic or; the caller clears it. */

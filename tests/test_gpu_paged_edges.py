@@ -194,3 +194,22 @@ def test_a_batch_that_lives_on_keeps_little(V):
         got = V.paged_attention(c.cache, c.batch, c.q, sliding_window=1000 + n, n_sinks=n)
         assert torch.equal(got, want)
     assert len(c.batch._workspace_bytes) <= 64
+
+
+@pytest.mark.parametrize("n", [5, 70])
+@pytest.mark.parametrize("what", ["cached", "order"])
+def test_append_reports_bad_sequences_without_tokens(V, n, what):
+    """As the attention does: also those that no token of the call belongs to."""
+    q_len = [1] * n
+    q_len[3] = 0
+    c = Case(V, torch, "bf16", 4, 2, 64, 8, q_len, [9] * n, seed=39, poison=False)
+    if what == "cached":
+        c.kv[3] = -4
+    else:
+        c.q_start[-1] = 0  # the last sequence ends before it begins
+    k = torch.zeros(c.tokens, 2, 64, device="cuda", dtype=torch.bfloat16)
+    V.paged_append_rope(c.cache, c.batch, k, k, 0.0)
+    assert int(c.status) == V.PAGED_BAD_LENGTH
+    c.status.zero_()
+    V.paged_attention(c.cache, c.batch, torch.zeros(c.tokens, 4, 64, device="cuda", dtype=torch.bfloat16))
+    assert int(c.status) == V.PAGED_BAD_LENGTH

@@ -53,7 +53,8 @@ __device__ __forceinline__ void append_store(T* p, const AppendUnit<T, WIDE>& u)
 }
 
 // Where token t goes; one warp calls it.  For up to 32 sequences every lane
-// takes one, so that all their numbers arrive together.
+// takes one, so that all their numbers arrive together.  (More sequences are
+// checked by the first CTA, whether a token belongs to them or not.)
 struct AppendPlace {
     int seq, p;
     int64_t first;
@@ -66,6 +67,7 @@ __device__ __forceinline__ AppendPlace append_place(const PagedAppendArgs& a, in
     if (a.n_seqs <= 32) {
         if (lane < a.n_seqs) {
             q = paged_seq(a, lane);
+            if (!q.ok) paged_status(a, VOX_PAGED_BAD_LENGTH);
             r.first = a.first_pos ? a.first_pos[lane] : 0;
         }
         const unsigned before = __ballot_sync(~0u, lane < a.n_seqs && q.q0 <= t);
@@ -82,7 +84,6 @@ __device__ __forceinline__ AppendPlace append_place(const PagedAppendArgs& a, in
         q = paged_seq(a, r.seq);
         r.first = a.first_pos ? a.first_pos[r.seq] : 0;
     }
-    if (!q.ok && lane == 0) paged_status(a, VOX_PAGED_BAD_LENGTH);
     r.stored_seq = q.ok && t - q.q0 < q.nq;  // else behind the last sequence, or skipped
     r.p = q.len - q.nq + (t - q.q0);
     return r;
@@ -113,6 +114,11 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const __grid_const
         }
     };
     load(h0);
+    if (blockIdx.x == 0 && a.n_seqs > 32) {
+        bool bad = false;
+        for (int s = threadIdx.x; s < a.n_seqs; s += 256) bad |= !paged_seq(a, s).ok;
+        if (bad) paged_status(a, VOX_PAGED_BAD_LENGTH);
+    }
 
     const AppendPlace at = append_place(a, t);
     if (!at.stored_seq) return;
