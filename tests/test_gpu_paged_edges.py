@@ -1,11 +1,12 @@
 """GPU tests of the paged-cache attention where single keys outweigh all others,
 where calls share what they should not, and where arguments are at their limits."""
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
 
-from tests.paged_testlib import Case
+from tests.paged_testlib import EPS_HALF, Case, torch_dtype
 from tests.vox_testlib import vox
 
 pytestmark = pytest.mark.gpu
@@ -152,7 +153,6 @@ def test_a_batch_serves_pools_of_different_page_sizes(V):
     with the same batch in between."""
     c = Case(V, torch, "bf16", 8, 2, 64, 16, (1, 2), (70, 90), seed=35)
     small = Case(V, torch, "bf16", 8, 2, 64, 8, (1,), (5,), seed=36)
-    import ctypes as C
     mine = C.cast(c.batch._for(c.cache), C.POINTER(V.PagedBatchDesc)).contents
     other = C.cast(c.batch._for(small.cache), C.POINTER(V.PagedBatchDesc)).contents
     width = c.table_dev.shape[1]
@@ -213,3 +213,57 @@ def test_append_reports_bad_sequences_without_tokens(V, n, what):
     c.status.zero_()
     V.paged_attention(c.cache, c.batch, torch.zeros(c.tokens, 4, 64, device="cuda", dtype=torch.bfloat16))
     assert int(c.status) == V.PAGED_BAD_LENGTH
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads,kv,dim,seqs,tokens", [(8, 2, 128, 3, 1185), (32, 8, 128, 40, 1300), (4, 1, 64, 1, 2400),
+                                                      (2, 2, 256, 1201, 1201)])
+def test_append_of_many_tokens(V, dtype, heads, kv, dim, seqs, tokens):
+    """From 1184 tokens on a block of threads takes two; the last one here has one
+    or two, and rows behind the last sequence stay."""
+    page, theta, base, spare = 16, 1e6, 70001, 2 if tokens % 2 == 0 else 3
+    cut = np.linspace(0, tokens, seqs + 1).astype(int)
+    q_len = np.diff(cut)
+    kv_len = q_len + np.arange(seqs) % 7
+    width = -(-int(kv_len.max()) // page)
+    rng = np.random.default_rng(40)
+    order = rng.permutation(seqs * width + 2).astype(np.int32)
+    table = order[:seqs * width].reshape(seqs, width)
+    shape = (len(order), kv, page, dim)
+    g = torch.Generator(device="cuda").manual_seed(41)
+    td = torch_dtype(dtype)
+    kp, vp = (torch.randn(shape, generator=g, device="cuda").to(td) for _ in range(2))
+    before = kp.clone(), vp.clone()
+    qkv = torch.randn(tokens + spare, heads + 2 * kv, dim, generator=g, device="cuda").to(td)
+    first = qkv.clone()
+    dev = dict(device="cuda")
+    batch = V.PagedBatch(torch.from_numpy(cut.astype(np.int32)).to(**dev), torch.from_numpy(kv_len.astype(np.int32)).to(**dev),
+                         torch.from_numpy(table).to(**dev), tokens + spare, int(q_len.max()),
+                         first_pos=torch.full((seqs,), base, dtype=torch.int64, device="cuda"))
+    q = qkv[:, :heads]
+    assert V.paged_append_rope(V.PagedKvCache(kp, vp), batch, qkv[:, heads:heads + kv], qkv[:, heads + kv:], theta, q=q,
+                               q_out=q) is q
+    batch.check()
+    assert torch.equal(qkv[tokens:], first[tokens:]) and torch.equal(qkv[:, heads:], first[:, heads:])
+    seq = np.repeat(np.arange(seqs), q_len)
+    index = kv_len[seq] - q_len[seq] + np.arange(tokens) - cut[seq]
+    ang = (base + index)[:, None] * theta ** (-np.arange(0, dim, 2) / dim)
+    cos, sin = (torch.from_numpy(f(ang)).cuda()[:, None] for f in (np.cos, np.sin))
+
+    def check(got, x):
+        x0, x1 = x[..., 0::2].double(), x[..., 1::2].double()
+        want = torch.stack((x0 * cos - x1 * sin, x0 * sin + x1 * cos), -1).flatten(-2)
+        size = (x0.abs() + x1.abs()).repeat_interleave(2, -1)
+        # a product and a sum of 32 bits and the angle's 2^-24, then one rounding to the type
+        over = (got.double() - want).abs() - (EPS_HALF[dtype] * want.abs() + size * 2.0 ** -21)
+        # below f16's normal range, 2^-14, half a step is 2^-25 and no longer 2^-11 of the
+        # value: of 17 million results three there were off by up to 2.2e-8 more
+        assert float(over.max()) <= (2.0 ** -25 if dtype == "f16" else 0)
+
+    check(q[:tokens], first[:tokens, :heads])
+    at = torch.from_numpy(table[seq, index // page].astype(np.int64)).cuda(), torch.from_numpy(index % page).cuda()
+    check(kp[at[0], :, at[1]], first[:tokens, heads:heads + kv])
+    assert torch.equal(vp[at[0], :, at[1]], first[:tokens, heads + kv:])
+    for pool, old in zip((kp, vp), before):
+        pool[at[0], :, at[1]] = old[at[0], :, at[1]]
+        assert torch.equal(pool, old)
