@@ -267,3 +267,67 @@ def test_append_of_many_tokens(V, dtype, heads, kv, dim, seqs, tokens):
     for pool, old in zip((kp, vp), before):
         pool[at[0], :, at[1]] = old[at[0], :, at[1]]
         assert torch.equal(pool, old)
+
+
+def timed(f, n=5):
+    f()
+    best = math.inf
+    for _ in range(n):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q_len,kv_len", [((300,), (3000,)), ((1,) * 16, (4000,) * 16)])
+@pytest.mark.parametrize("bad", [1, 40, 1000])
+def test_rows_that_see_a_nan_cost_little(V, dtype, q_len, kv_len, bad):
+    """They are NaN at once: only rows that do not see what is not finite beside
+    their keys are worth doing again.  (Done again they took 20 to 260 times as long.)"""
+    c = Case(V, torch, dtype, 8, 2, 128, 16, q_len, kv_len, seed=42, poison=False)
+    want, clean = c.run(), timed(c.run)
+    pages = torch.from_numpy(c.table[:, :bad // 16 + 1].astype(np.int64)).cuda()
+    for s in range(c.n):
+        c.vp[pages[s], :, :min(bad, 16), 7] = math.nan
+    got = c.run()
+    assert bool(torch.isnan(got[..., 7]).all())
+    keep = [d for d in range(128) if d != 7]
+    assert torch.equal(got[..., keep], want[..., keep])
+    took = timed(c.run)
+    assert took < 8 * clean
+    c.kp[pages[0], 0, 0, 0] = math.nan  # and no scores
+    assert bool(torch.isnan(c.run()[:q_len[0], :4]).all())
+    assert timed(c.run) < 8 * clean
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("prefix", [0, 50])
+@pytest.mark.parametrize("q_len,kv_len,window,sinks", [((90,), (400,), 0, 0), ((200, 3), (300, 60), 100, 4), ((1, 5), (300, 200), 64, 2)])
+def test_many_values_that_are_not_finite(V, dtype, prefix, q_len, kv_len, window, sinks):
+    """Values of 60 keys, of every kind, in and out of sight: each row has what its
+    own keys add up to."""
+    c = Case(V, torch, dtype, 8, 2, 64, 16, q_len, kv_len, window, sinks, prefix=prefix, seed=43, poison=False)
+    rng = np.random.default_rng(44)
+    for s in range(c.n):
+        for i, j in enumerate(rng.permutation(kv_len[s])[:60]):
+            c.v[s][j, i % 2, rng.integers(20)] = (math.nan, math.inf, -math.inf)[i % 3]
+    for i in range(0, prefix, 9):
+        c.pv[i, i % 2, rng.integers(20, 30)] = (math.inf, math.nan)[i % 2]
+    live = c.table >= 0
+    for s in range(c.n):
+        for j in range(kv_len[s]):
+            if live[s, j // 16]:
+                c.vp[c.table[s, j // 16], :, j % 16] = c.v[s][j].cuda()
+    for j in range(prefix):
+        if c.pre[j // 16] >= 0:
+            c.vp[c.pre[j // 16], :, j % 16] = c.pv[j].cuda()
+    got = c.run().float().cpu().numpy()
+    want, tol = c.expected()
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isposinf(got), np.isposinf(want))
+    ok = np.isfinite(want)
+    assert np.array_equal(np.isneginf(got), np.isneginf(want)) and ok.any() and not ok.all()
+    assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])

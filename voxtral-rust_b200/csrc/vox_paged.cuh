@@ -167,12 +167,102 @@ __device__ __forceinline__ int64_t paged_row(const PagedAttnArgs& a, const Paged
     return page * a.page_stride + h * a.head_stride + ks.slot(j, a.page_shift) * a.slot_stride;
 }
 
-// One row again, key by key: acc[e] = sum of 2^(score - m) v[lane + 32 e] over
-// the keys that the row sees among blocks b0..b1-1 of `keys` keys.  For rows
-// whose result is not finite; one warp calls it.
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < __builtin_huge_valf()); }
+
+// ---- rows whose result is not finite ----
+//
+// A masked weight is 0, but 0 x inf is NaN: a result that is not finite may come from
+// a value that the row does not see.  Where a CTA meets one, its warps list the keys
+// among its own whose values are not all finite (paged_find_odd).  A row whose every
+// such result has a value of a key that it sees behind it has the sum of those
+// (paged_explain_row); one with a result that none explains is done again key by key
+// (paged_redo_row).  A row whose sum of weights is NaN is NaN, whatever the values.
+
+// (All inlined: a call anywhere in the tcgen05 kernel costs its loop 2 to 5 %.)
+
+// A CTA's keys: blocks b0..b1-1 of those in kb, of kv head h.
+struct PagedShare {
+    PagedKeys ks;
+    KeyBlocks kb;
+    int b0, b1, h;
+};
+// Those with values that are not finite; more than fit are counted and left out.
+constexpr int kPagedOddKeys = 32;
+struct PagedOdd {
+    int n, key[kPagedOddKeys];
+};
+
+// Lists the keys (odd->n is 0 before); blocks are of `keys` keys, and warp `warp` of
+// `warps` takes its share.
 template <class T, int E>
-__device__ __noinline__ void paged_redo_row(const PagedAttnArgs& a, PagedKeys ks, KeyBlocks kb, int keys, int b0, int b1,
-                                            int h, int tok, int head, int p, float m, float (&acc)[E]) {
+__device__ __forceinline__ void paged_find_odd(const PagedAttnArgs& a, const PagedShare& c, PagedOdd* odd, int keys, int warp,
+                                               int warps) {
+    constexpr int U = 4;  // keys at once
+    const int lane = threadIdx.x & 31, total = (c.b1 - c.b0) * keys;
+#pragma unroll 1
+    for (int i0 = warp * U; i0 < total; i0 += warps * U) {
+        int j[U];
+        bool bad[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u;
+            j[u] = c.kb.block(c.b0 + i / keys) * keys + i % keys;
+            bad[u] = false;
+            if (i < total && c.kb.seen(j[u])) {
+                const int64_t off = paged_row(a, c.ks, j[u], c.h);
+                if (off >= 0) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) bad[u] |= not_finite(to_f32(static_cast<const T*>(a.v)[off + lane + 32 * e]));
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (__any_sync(~0u, bad[u]) && lane == 0) {
+                const int at = atomicAdd(&odd->n, 1);
+                if (at < kPagedOddKeys) odd->key[at] = j[u];
+            }
+    }
+}
+
+// acc[e]: element lane + 32 e of the result of a row with index p.  Where the row
+// sees values there that are not finite it becomes their sum (in any order the
+// same).  Whether that explains all of them; one warp calls it.
+template <class T, int E>
+__device__ __forceinline__ bool paged_explain_row(const PagedAttnArgs& a, const PagedShare& c, const PagedOdd* odd, int p,
+                                                  float (&acc)[E]) {
+    const int lane = threadIdx.x & 31, n = min(odd->n, kPagedOddKeys);
+    float sum[E] = {};
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const int j = odd->key[i];
+        if (!paged_sees(p, j, c.ks.len, a.window, c.ks.sinks)) continue;
+        const int64_t off = paged_row(a, c.ks, j, c.h);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float v = to_f32(static_cast<const T*>(a.v)[off + lane + 32 * e]);
+            if (not_finite(v)) sum[e] += v;
+        }
+        bool more = false;  // (NaN stays NaN)
+#pragma unroll
+        for (int e = 0; e < E; ++e) more |= not_finite(acc[e]) && sum[e] == sum[e];
+        if (!__any_sync(~0u, more)) break;
+    }
+    bool open = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        // (a key that is not listed could turn an infinity into NaN)
+        open |= not_finite(sum[e]) ? odd->n > n && sum[e] == sum[e] : not_finite(acc[e]);
+        if (not_finite(sum[e])) acc[e] = sum[e];
+    }
+    return !__any_sync(~0u, open);
+}
+
+// One row again, key by key: acc[e] = sum of 2^(score - m) v[lane + 32 e] over
+// the keys that the row sees, in blocks of `keys` keys; one warp calls it.
+template <class T, int E>
+__device__ __forceinline__ void paged_redo_row(const PagedAttnArgs& a, const PagedShare& c, int keys, int tok, int head, int p,
+                                               float m, float (&acc)[E]) {
     const int lane = threadIdx.x & 31;
     float q[E];
 #pragma unroll
@@ -181,21 +271,35 @@ __device__ __noinline__ void paged_redo_row(const PagedAttnArgs& a, PagedKeys ks
         acc[e] = 0.f;
     }
     const float base = m == kNegInf ? 0.f : m;
-    for (int b = b0; b < b1; ++b)
-        for (int i = 0; i < keys; ++i) {
-            const int j = kb.block(b) * keys + i;
-            if (!paged_sees(p, j, ks.len, a.window, ks.sinks)) continue;
-            const int64_t off = paged_row(a, ks, j, h);
-            if (off < 0) continue;  // zeros: adds nothing
-            float s = 0.f;
+    constexpr int U = 4;  // keys at once
+#pragma unroll 1
+    for (int i0 = 0, total = (c.b1 - c.b0) * keys; i0 < total; i0 += U) {
+        float s[U], v[U][E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f32(static_cast<const T*>(a.k)[off + lane + 32 * e]), s);
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-            const float w = fast_exp2(s * a.scale_log2 - base);
+        for (int u = 0; u < U; ++u) {
+            const int j = c.kb.block(c.b0 + (i0 + u) / keys) * keys + (i0 + u) % keys;
+            const int64_t off = i0 + u < total && paged_sees(p, j, c.ks.len, a.window, c.ks.sinks) ? paged_row(a, c.ks, j, c.h) : -1;
+            s[u] = off < 0 ? kNegInf : 0.f;  // a bad page: zeros, add nothing
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                v[u][e] = 0.f;
+                if (off >= 0) {
+                    s[u] = fmaf(q[e], to_f32(static_cast<const T*>(a.k)[off + lane + 32 * e]), s[u]);
+                    v[u][e] = to_f32(static_cast<const T*>(a.v)[off + lane + 32 * e]);
+                }
+            }
+        }
+        for (int o = 16; o; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(~0u, s[u], o);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = fast_exp2(s[u] * a.scale_log2 - base);
             if (w == 0.f) continue;
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, to_f32(static_cast<const T*>(a.v)[off + lane + 32 * e]), acc[e]);
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
         }
+    }
 }
 
 // A tile's query rows, up to 32: lane r of every warp has row r's token (-1: no

@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
     __shared__ float m_s[kWarps][ROWS], l_s[kWarps][ROWS], cm_s[ROWS], cl_s[ROWS];
     __shared__ float wc_s[16][ROWS], tot_s[ROWS];
     __shared__ int odd_s[ROWS];
+    __shared__ PagedOdd odd_keys;
     float* body = reinterpret_cast<float*>(smem);
     uint4* qf = reinterpret_cast<uint4*>(smem + Cfg::BODY);
 
@@ -469,8 +470,10 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
         cl_s[tid] = sum;
         odd_s[tid] = 0;
     }
+    if (tid == 0) odd_keys.n = 0;
     __syncthreads();
     constexpr int V4 = HD / 4;
+    bool odd = false;
     for (int i = tid; i < ROWS * V4; i += kThreads) {
         const int r = i / V4, d = (i % V4) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -480,18 +483,23 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
         }
         *reinterpret_cast<float4*>(body + r * OS + d) = v;
-        const float sum = (v.x + v.y) + (v.z + v.w);
-        if (!(fabsf(sum) < __builtin_huge_valf())) odd_s[r] = 1;
+        if (not_finite((v.x + v.y) + (v.z + v.w)) && tok_s[r] >= 0 && cl_s[r] == cl_s[r]) odd_s[r] = odd = true;
     }
-    __syncthreads();
-    // A value that is not finite may have come from a key that a row does not
-    // see (0 x inf): such rows are done again key by key.
-    for (int r = warp; r < ROWS; r += kWarps) {
-        if (!odd_s[r] || tok_s[r] < 0) continue;
-        float acc[HD / 32];
-        paged_redo_row<T, HD / 32>(a, ks, kb, kKeys, b0, b1, h, tok_s[r], head_s[r], p_s[r], cm_s[r], acc);
+    if (__syncthreads_or(odd)) {
+        const PagedShare mine{ks, kb, b0, b1, h};
+        paged_find_odd<T, HD / 32>(a, mine, &odd_keys, kKeys, warp, kWarps);
+        __syncthreads();
+#pragma unroll 1
+        for (int r = warp; r < ROWS; r += kWarps) {
+            if (!odd_s[r]) continue;
+            float acc[HD / 32];
 #pragma unroll
-        for (int e = 0; e < HD / 32; ++e) body[r * OS + lane + 32 * e] = acc[e];
+            for (int e = 0; e < HD / 32; ++e) acc[e] = body[r * OS + lane + 32 * e];
+            if (!paged_explain_row<T, HD / 32>(a, mine, &odd_keys, p_s[r], acc))
+                paged_redo_row<T, HD / 32>(a, mine, kKeys, tok_s[r], head_s[r], p_s[r], cm_s[r], acc);
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) body[r * OS + lane + 32 * e] = acc[e];
+        }
     }
 
     // ---- the cluster's, or this CTA's, result ----

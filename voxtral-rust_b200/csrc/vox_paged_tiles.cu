@@ -64,6 +64,7 @@ namespace {
 constexpr int kTile = 128;  // query rows of a tile, keys of a block
 constexpr int kTileThreads = 352;
 constexpr int kStep = 64;         // keys of a softmax step
+constexpr int kStageBytes = 32 * 128;  // a softmax warp's results on their way out
 // Log2 of the weight at a row's maximum when the reference is set by it, and the
 // sums of a step's weights above and (f16) below which the reference moves.
 template <class T>
@@ -276,7 +277,52 @@ struct TilesShared {
     uint32_t tmem;
     int lo[8], hi[8];  // smallest and largest index of a warp's rows
     int failed;
+    // for rows that are not finite (here, so that no register holds it meanwhile)
+    PagedShare share;
+    PagedOdd odd;
+    unsigned odd_lanes[8];
 };
+
+// A row whose result, already written, is not finite (paged_find_odd).
+struct OddRow {
+    int64_t at;  // where the result begins
+    int tok, head, p;
+    float m, inv;
+};
+// The CTA's odd rows; all its warps call it.  Softmax warp w has left those of its
+// lanes in `lanes[w]` where it staged its results, in the memory of its tile's queries.
+template <class T, int HD>
+__device__ __forceinline__ void tiles_mend_rows(const PagedAttnArgs& a, const PagedShare& share, PagedOdd* list,
+                                                const unsigned* lanes, const unsigned char* queries, bool to_part) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    paged_find_odd<T, HD / 32>(a, share, list, kTile, warp, kTileThreads / 32);
+    __syncthreads();
+    if (warp >= 8) return;
+    const OddRow* rows = reinterpret_cast<const OddRow*>(queries + (warp >> 2) * TilesCfg<HD>::TILE_BYTES + (warp & 3) * kStageBytes);
+#pragma unroll 1
+    for (unsigned todo = lanes[warp]; todo; todo &= todo - 1) {
+        const OddRow r = rows[__ffs(todo) - 1];
+        float acc[HD / 32];
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) {
+            const int64_t at = r.at + lane + 32 * e;
+            acc[e] = to_part ? a.part_o[at] : to_f32(static_cast<T*>(a.out)[at]);
+        }
+        if (!paged_explain_row<T, HD / 32>(a, share, list, r.p, acc)) {
+            paged_redo_row<T, HD / 32>(a, share, kTile, r.tok, r.head, r.p, r.m, acc);
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) acc[e] *= to_part ? 1.f : r.inv;
+        }
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) {
+            const int64_t at = r.at + lane + 32 * e;
+            if (to_part)
+                a.part_o[at] = acc[e];
+            else
+                static_cast<T*>(a.out)[at] = from_f32<T>(acc[e]);
+        }
+    }
+}
 
 template <class T, int HD>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -412,9 +458,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         n -= b0;
     }
 
+    if (tid == 0) sh.share = PagedShare{ks, kb, b0, b0 + n, h}, sh.odd.n = 0;
+
     // Bounded waits: of a thread, and of a whole warp with one answer.
     auto wait = [&](uint64_t* bar, uint32_t parity) { return tiles_wait(bar, parity, a.wait_polls); };
     auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(~0u, wait(bar, parity)); };
+    bool odd = false;
     if (warp == 10) {
         // ---- K and V tiles ----
         const int ps = 1 << a.page_shift;
@@ -609,11 +658,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const bool write = ok && tok >= 0;
         if (to_part && write) a.part_ml[at] = make_float2(m, l);
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        bool odd = false;
         // The rows go through the tile's queries' memory (all products with them are
         // done), 32 floats or 64 results of a row at a time, so that a store covers
         // 128 bytes of a row; the 16-byte columns are swizzled by the row.
-        const uint32_t stage = q_sm + t * Cfg::TILE_BYTES + (warp & 3) * (32 * 128);
+        const uint32_t stage = q_sm + t * Cfg::TILE_BYTES + (warp & 3) * kStageBytes;
         const int64_t row_at = to_part ? at * HD : tok * a.o_ts + head * a.o_hs;
         const int width = to_part ? 32 : 64;  // elements of 128 bytes
         if (ok) {
@@ -631,7 +679,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     float check = 0.f;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) check += fabsf(__uint_as_float(o[e]));
-                    odd |= !(check < __builtin_huge_valf());
+                    odd |= not_finite(check);
                     if (!to_part) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
@@ -666,27 +714,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 __syncwarp();
             }
         }
-        // A value that is not finite may have come from a key that the row does
-        // not see (0 x inf): such rows are done again key by key.
-        __syncwarp();
-        for (unsigned todo = __ballot_sync(~0u, odd && write); todo; todo &= todo - 1) {
-            const int src = __ffs(todo) - 1;
-            const int rt = __shfl_sync(~0u, tok, src), rh = __shfl_sync(~0u, head, src), rp = __shfl_sync(~0u, p, src);
-            const float rm = __shfl_sync(~0u, m, src), ri = __shfl_sync(~0u, inv, src);
-            float acc[HD / 32];
-            paged_redo_row<T, HD / 32>(a, ks, kb, kTile, b0, b0 + n, h, rt, rh, rp, rm, acc);
-            const int64_t ra = __shfl_sync(~0u, at, src);
-#pragma unroll
-            for (int e = 0; e < HD / 32; ++e) {
-                if (to_part)
-                    a.part_o[ra * HD + lane + 32 * e] = acc[e];
-                else
-                    static_cast<T*>(a.out)[rt * a.o_ts + rh * a.o_hs + lane + 32 * e] = from_f32<T>(acc[e] * ri);
-            }
-        }
+        // (what is left of a row is kept where its warp staged the results)
+        odd = odd && write && l == l;
+        const unsigned lanes_odd = __ballot_sync(~0u, odd);
+        if (lane == 0) sh.odd_lanes[warp] = lanes_odd;
+        if (odd) reinterpret_cast<OddRow*>(smem_raw + (stage - smem_addr(smem_raw)))[lane] = OddRow{row_at, tok, head, p, m, inv};
         tmem_fence_before();
     }
-    __syncthreads();
+    if (__syncthreads_or(odd))
+        tiles_mend_rows<T, HD>(a, sh.share, &sh.odd, sh.odd_lanes, smem_raw + (q_sm - smem_addr(smem_raw)), to_part);
     if (tid == 0 && sh.failed) paged_status(a, VOX_PAGED_TIMEOUT);
     if (warp == 8) {
         tmem_fence_after();
