@@ -76,3 +76,10 @@ def test_scales_that_overflow_are_refused(V):
     L = V.lib()
     refused(V, L.vox_paged_attention(c, b, r, 4, 0, 0, 3e38, r, None, 0, None), "ERR_INVALID_ARG", "scale")
     refused(V, L.vox_paged_prefix_attention(c, b, p, r, 4, 0, 0, 3e38, r, None, 0, None), "ERR_INVALID_ARG", "scale")
+
+
+def test_append_refuses_rotated_queries_without_queries(V):
+    c, b, _, r = (C.byref(x) for x in descs(V))
+    refused(V, V.lib().vox_paged_append_rope(c, b, r, r, 1e4, 4, None, r, None), "ERR_INVALID_ARG", "q_out")
+    with pytest.raises(ValueError, match="q_out needs q"):
+        V.paged_append_rope(None, None, None, None, 1e4, q_out=object())

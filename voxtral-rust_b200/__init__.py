@@ -1294,6 +1294,8 @@ def paged_append_rope(cache: PagedKvCache, batch: PagedBatch, k_new, v_new, rope
     their positions; queries [n_tokens, n_heads, head_dim], if given, rotated
     into q_out (a new tensor by default; q itself is fine), which is returned.
     rope_theta 0: no rotation (vox_paged_append_rope)."""
+    if q is None and q_out is not None:
+        raise ValueError("q_out needs q")
     torch, stream, L = _paged_env()
     ref = batch._for(cache)
     k = _paged_rows(k_new, "k_new", batch, cache.n_kv_heads, cache)

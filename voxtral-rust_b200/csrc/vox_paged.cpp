@@ -436,6 +436,7 @@ extern "C" int vox_paged_append_rope(const vox_paged_cache* c, const vox_paged_b
     TRY(check_batch(c, b));
     if (theta != 0.f && !(theta >= 1.f && std::isfinite(theta)))
         return report_errorf(VOX_ERR_INVALID_ARG, "rope_theta must be 0 or finite and >= 1");
+    if (!q && q_out) return report_errorf(VOX_ERR_INVALID_ARG, "null q beside q_out");
     if (q && (n_heads == 0 || n_heads > 65536)) return report_errorf(VOX_ERR_INVALID_ARG, "n_heads must be in 1..65536");
     if (b->n_seqs == 0 || b->n_tokens == 0) return VOX_OK;
     if (!rows_apart({{c->n_pages, (size_t)k.page_stride}, {c->n_kv_heads, (size_t)k.head_stride}, {c->page_size, (size_t)k.slot_stride}},
