@@ -331,3 +331,26 @@ def test_many_values_that_are_not_finite(V, dtype, prefix, q_len, kv_len, window
     ok = np.isfinite(want)
     assert np.array_equal(np.isneginf(got), np.isneginf(want)) and ok.any() and not ok.all()
     assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 4, 70])
+def test_keys_with_an_infinity(V, dtype, n):
+    """A seen key whose score is -inf has no weight; the rows whose score with it is
+    +inf are NaN."""
+    c = Case(V, torch, dtype, 4, 1, 64, 16, (n,), (n + 300,), seed=45, poison=False)
+    c.q_host[..., 5] = c.q_host[..., 5].abs() + 0.25
+    c.q_host[-1, 1, 5] *= -1
+    c.q = c.q_host.cuda()
+    for j in (0, 77, 200):
+        # as good as -inf to 64 bits too: a score of -300 and less
+        c.k[0][j, 0, 5] = -10000.0
+        c.kp[c.table[0, j // 16], 0, j % 16] = c.k[0][j, 0].cuda()
+        c.kp[c.table[0, j // 16], 0, j % 16, 5] = -math.inf
+    got = c.run()
+    assert bool(torch.isnan(got[-1, 1]).all())
+    got[-1, 1] = 0
+    assert bool(torch.isfinite(got).all())
+    want, tol = c.expected()
+    want[-1, 1] = 0
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)

@@ -176,7 +176,8 @@ __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < __buil
 // among its own whose values are not all finite (paged_find_odd).  A row whose every
 // such result has a value of a key that it sees behind it has the sum of those
 // (paged_explain_row); one with a result that none explains is done again key by key
-// (paged_redo_row).  A row whose sum of weights is NaN is NaN, whatever the values.
+// (paged_redo_row).  A row whose sum of weights is NaN is NaN, whatever the values (of
+// f32 see paged_rescore_row).
 
 // (All inlined: a call anywhere in the tcgen05 kernel costs its loop 2 to 5 %.)
 
@@ -300,6 +301,44 @@ __device__ __forceinline__ void paged_redo_row(const PagedAttnArgs& a, const Pag
             for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[u][e], acc[e]);
         }
     }
+}
+
+// One f32 row again with its scores: the halves of a key's or a query's infinity
+// multiply to NaN where the score itself is an infinity (one that is -inf has no
+// weight).  Sets the reference m, the sum l and acc; NaN where a score is.
+template <int E>
+__device__ __forceinline__ void paged_rescore_row(const PagedAttnArgs& a, const PagedShare& c, int keys, int tok, int head, int p,
+                                                  float* m, float* l, float (&acc)[E]) {
+    const int lane = threadIdx.x & 31;
+    float q[E], top = kNegInf, sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        q[e] = static_cast<const float*>(a.q)[tok * a.q_ts + head * a.q_hs + lane + 32 * e];
+        acc[e] = 0.f;
+    }
+#pragma unroll 1
+    for (int i = 0, total = (c.b1 - c.b0) * keys; i < total && sum == sum; ++i) {
+        const int j = c.kb.block(c.b0 + i / keys) * keys + i % keys;
+        if (!paged_sees(p, j, c.ks.len, a.window, c.ks.sinks)) continue;
+        const int64_t off = paged_row(a, c.ks, j, c.h);
+        float s = 0.f;
+        if (off >= 0)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s = fmaf(q[e], static_cast<const float*>(a.k)[off + lane + 32 * e], s);
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+        s *= a.scale_log2;
+        if (s == kNegInf) continue;
+        const float now = fmaxf(top, s), f = fast_exp2(top - now), w = fast_exp2(s - now);
+        sum = sum * f + w;
+        top = now;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float v = off >= 0 ? static_cast<const float*>(a.v)[off + lane + 32 * e] : 0.f;
+            acc[e] = w == 0.f ? acc[e] * f : fmaf(w, v, acc[e] * f);
+        }
+    }
+    *m = top;
+    *l = sum;
 }
 
 // A tile's query rows, up to 32: lane r of every warp has row r's token (-1: no

@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
         }
         *reinterpret_cast<float4*>(body + r * OS + d) = v;
-        if (not_finite((v.x + v.y) + (v.z + v.w)) && tok_s[r] >= 0 && cl_s[r] == cl_s[r]) odd_s[r] = odd = true;
+        if (not_finite((v.x + v.y) + (v.z + v.w)) && tok_s[r] >= 0 && (F32 || cl_s[r] == cl_s[r])) odd_s[r] = odd = true;
     }
     if (__syncthreads_or(odd)) {
         const PagedShare mine{ks, kb, b0, b1, h};
@@ -495,11 +495,17 @@ __global__ void __launch_bounds__(32 * RowsCfg<T, HD, NT>::WARPS, RowsCfg<T, HD,
             float acc[HD / 32];
 #pragma unroll
             for (int e = 0; e < HD / 32; ++e) acc[e] = body[r * OS + lane + 32 * e];
-            if (!paged_explain_row<T, HD / 32>(a, mine, &odd_keys, p_s[r], acc))
+            if (F32 && cl_s[r] != cl_s[r]) {
+                float m_new, l_new;
+                paged_rescore_row<HD / 32>(a, mine, kKeys, tok_s[r], head_s[r], p_s[r], &m_new, &l_new, acc);
+                __syncwarp();
+                if (lane == 0) cm_s[r] = m_new, cl_s[r] = l_new;
+            } else if (!paged_explain_row<T, HD / 32>(a, mine, &odd_keys, p_s[r], acc))
                 paged_redo_row<T, HD / 32>(a, mine, kKeys, tok_s[r], head_s[r], p_s[r], cm_s[r], acc);
 #pragma unroll
             for (int e = 0; e < HD / 32; ++e) body[r * OS + lane + 32 * e] = acc[e];
         }
+        __syncthreads();
     }
 
     // ---- the cluster's, or this CTA's, result ----
