@@ -354,3 +354,16 @@ def test_keys_with_an_infinity(V, dtype, n):
     want, tol = c.expected()
     want[-1, 1] = 0
     assert np.all(np.abs(got.double().cpu().numpy() - want) <= tol)
+
+
+@pytest.mark.parametrize("step", [12.0, 25.0, 40.0, 70.0])
+def test_scores_that_fall_again_and_again(V, step):
+    """Every 64 keys far below the ones before, by up to 70 nats: the first, of value
+    0, has all of the weight to 32 bits, and what follows adds up or is lost below the
+    results' range, but nothing overflows."""
+    c = dominated(V, "f16", 0.0, 0.0, (), heads=4, kv_heads=1, dim=128, q_len=(20,), kv_len=(1000,), seed=46)
+    for i in range(0, 1000, 64):
+        c.k[0][i:i + 64, :, 0] = max(300.0 - step * (i // 64), -300.0) * math.sqrt(c.dim) / 8.0
+    c.v[0][:64] = 0.0
+    store(c)
+    check_dominated(c, c.run())

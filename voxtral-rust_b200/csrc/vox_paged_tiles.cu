@@ -71,6 +71,7 @@ template <class T>
 struct TilesRange {
     static constexpr bool F16 = std::is_same<T, __half>::value;
     static constexpr float TOP = F16 ? 8.f : 0.f, RISE = F16 ? 65504.f : 256.f, FALL = 0x1p-4f;
+    static constexpr uint32_t LEAST = (127u - 60u) << 23;  // 2^-60's bits: sums below are not looked at
 };
 constexpr uint32_t kTmemO = 0, kTmemS = 256, kTmemCols = 512;  // S_t buffer b at kTmemS + (2 t + b) 64
 
@@ -610,19 +611,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                              (a.window == 0 || j0 > pmax - a.window || j0 + kStep <= ks.sinks);
             tmem_ld64(buf, s);
             if (!all) tiles_mask(s, p - j0, ks.len - j0, a.window, ks.sinks - j0);
-            // The weights are taken with the reference so far.  Only where their sum says
-            // that a score may have risen far above it (the first steps, mostly), or for
-            // f16 that all are far below it, is the maximum looked for and the weights
-            // taken again.  (Weights of less than 2^-80 of the sum so far stay as they are:
-            // the sums' range is f32's.)
+            // The weights are taken with the reference so far, and are on their way before
+            // it is known whether that was right.  Only where their sum says that a score
+            // may have risen far above it (the first steps, mostly), or for f16 that all are
+            // far below it (2^-60 of it and more: the sums' range is f32's), is the maximum
+            // looked for and the weights taken again.
             float l_new = 0.f;
-            if (k > 0) l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
-            const bool fell = Range::F16 && l_new < Range::FALL && l_new * 0x1p80f > l;
+            if (k > 0) {
+                l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
+                tmem_st32(buf, w);
+            }
+            bool fell = Range::F16 && __float_as_uint(l_new) - Range::LEAST < __float_as_uint(Range::FALL) - Range::LEAST;
             if (k == 0 || __any_sync(~0u, l_new > Range::RISE || m == kNegInf || fell)) {
+                tmem_wait_st();
                 float mx = kNegInf;
 #pragma unroll
                 for (int c = 0; c < kStep; c += 2) mx = max3(mx, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                const float want = mx * a.scale_log2 - Range::TOP, m_new = fell ? want : fmaxf(m, want);
+                const float want = mx * a.scale_log2 - Range::TOP;
+                if constexpr (Range::F16) fell = fell && l * fast_exp2(m - want) < 0x1p90f;
+                const float m_new = fell ? want : fmaxf(m, want);
                 const float f = m_new == kNegInf ? 1.f : fast_exp2(m - m_new);
                 m = m_new;
                 l *= f;
@@ -640,9 +647,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
                 l_new = tiles_weights<T>(s, w, a.scale_log2, m == kNegInf ? 0.f : -m);
+                tmem_st32(buf, w);
             }
             l += l_new;
-            tmem_st32(buf, w);
             tmem_wait_st();
             tmem_fence_before();
             __syncwarp();
