@@ -640,8 +640,13 @@ int vox_paged_append_rope(const vox_paged_cache* cache, const vox_paged_batch* b
  * 0 (as in vox_attention_gqa_step).  A token that sees nothing gets zeros.
  * Keys and values that a token does not see do not affect it, whatever they
  * hold; page ids that no token needs are not looked at.  scale 0 =
- * 1/sqrt(head_dim).  f16 and bf16 tensors are multiplied as they are and
- * accumulated in f32.  `out` must not overlap q or the pool.  `workspace` is
+ * 1/sqrt(head_dim).  All sums are f32.  f16 and bf16 keys and queries are
+ * multiplied as they are; the softmax's weights are rounded to the type, each by
+ * at most half a step of its own (f16: or 2^-33 of the largest, for keys that have
+ * less than 2^-22 of a near one's weight).  f32 tensors are multiplied in tf32
+ * halves, without the product of the two lower ones (2^-22 of a product).  (Both at
+ * head_dim 64 and 128 with rows on 16-byte boundaries; otherwise in f32 as they
+ * are.)  `out` must not overlap q or the pool.  `workspace` is
  * scratch memory of the size that vox_paged_attention_workspace gives (it may
  * be 0), 256-byte aligned; calls that can overlap on the GPU need one each. */
 int vox_paged_attention_workspace(const vox_paged_cache* cache, const vox_paged_batch* batch, size_t n_heads,
@@ -650,8 +655,10 @@ int vox_paged_attention(const vox_paged_cache* cache, const vox_paged_batch* bat
                         size_t n_heads, size_t sliding_window, size_t n_sinks, float scale, const vox_rows* out,
                         void* workspace, size_t workspace_bytes, void* stream);
 /* The same for a batch whose sequences all begin with one shared prefix,
- * which is read from memory once for all of them (and multiplied once, unless
- * it is so short that reading it out of the L2 for every sequence is faster):
+ * which is read once for each tile of query rows of all of them (256 rows of f16
+ * and bf16 with head_dim 64 or 128, pages of 8 slots and more, and rows on 16-byte
+ * boundaries; at most 32 otherwise), or, where it is so short that this is faster,
+ * for each sequence, out of the L2 where it fits:
  * *prefix_len tokens (a device int32, at most max_len) in the pages
  * prefix->pages [n_pages].  The batch's table, kv_len and bounds are those of
  * the sequences' own tokens behind the prefix; a token's index, for the window

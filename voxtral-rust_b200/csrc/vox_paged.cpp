@@ -236,8 +236,8 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
             if (z == 1 || t < best) best = t, p.splits = (int)z;
         }
         // A last wave that leaves at least half of the SMs empty: only its tiles are
-        // split, over all SMs (512 tiles of 65 blocks, 3.46 waves: 487 us instead of
-        // 528); joining them costs about 2 blocks' time.
+        // split, over all SMs (512 tiles of 65 blocks, 3.46 waves: 508 us in a CUDA
+        // graph instead of 553); joining them costs about 2 blocks' time.
         const int64_t last = units % 148;
         if (alike && units > 148 && last > 0 && last <= 74) {
             const int64_t z = std::min<int64_t>(148 / last, blocks / 2);
@@ -252,12 +252,12 @@ KeysPlan plan_keys(const vox_paged_cache* c, PagedType t, int64_t rows, int64_t 
     // CTAs that run at once.  Fewer tiles than that are split into one wave of
     // equal parts; more, where the bytes bound the call (one decode step's rows),
     // into about eight waves, which evens out ragged lengths: 96 sequences of up
-    // to 8192 visible keys 402 us against 408 with two CTAs a tile.
+    // to 8192 visible keys 400 us in a CUDA graph, 413 with two CTAs a tile.
     const int64_t slots = 148 * (p.nt == 1 ? 3 : 2);
     const int64_t wanted = units < slots ? slots / units : p.nt == 1 ? (8 * slots + units - 1) / units : 1;
     // At least 64 keys to a CTA of a cluster, 512 where there are enough tiles
     // without, or where the parts go through the merge (one stream of 1536 tokens:
-    // 15 us a call through clusters alone, 20 us with a merge behind them).
+    // 8.5 us in a CUDA graph through clusters alone, 9.6 with a merge behind them).
     int64_t parts = std::max<int64_t>(1, std::min<int64_t>(wanted, keys / (units < slots ? 64 : 512)));
     if (fits)
         while (p.cluster < 16 && 2 * p.cluster <= parts) p.cluster *= 2;
@@ -290,7 +290,7 @@ AttnPlan plan_attention(const vox_paged_cache* c, PagedType t, const vox_paged_b
     const int64_t rows = (int64_t)b->max_q_len * group;
     // A short prefix is read again for every sequence, out of the L2, as the first
     // part of its keys: one launch where the shared form takes three (8 hypotheses
-    // behind 639 tokens: 10 us against 17).  32 MB are about 4 us of it.
+    // behind 639 tokens: 10 us in a CUDA graph against 19).  32 MB are about 4 us of it.
     plan.joined = p && rows <= 32 &&
                   (double)b->n_seqs * (double)p->max_len * (double)(c->n_kv_heads * c->head_dim * 2 * type_size(t)) <= 32e6;
     const int64_t keys = visible(b->max_kv_len + (plan.joined ? p->max_len : 0));

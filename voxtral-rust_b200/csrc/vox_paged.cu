@@ -14,9 +14,9 @@ namespace {
 // pairs' sines and cosines are computed once, then it walks over the heads of k, v
 // and q with up to 6 rows in flight, loaded before it is known where the token
 // goes.  A CTA of 256 threads takes 2 tokens where there are many (fewer sines; one
-// round of loads for 32 + 16 heads of 128: 8.8k tokens 59 us, 4.3 TB/s, against 62
+// round of loads for 32 + 16 heads of 128: 8.8k tokens 58 us, 4.3 TB/s, against 62
 // with 4 tokens and two rounds, 81 with one), and one where there are few (all
-// heads at once: a single token 3.4 us in a graph).
+// heads at once: a single token 3.3 us; all in a CUDA graph).
 //
 // The angle a * theta^(-2c/D) matters modulo a turn only.  turns[c] is the turn
 // fraction per position as a 64-bit binary fraction, so the 64-bit product with

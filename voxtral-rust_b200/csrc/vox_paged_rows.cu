@@ -18,10 +18,10 @@
 // the exponents of f32; f16 weights are taken as 2^15 times what they are beside the
 // maximum, so that they keep all their bits down to 2^-29 of it (18 nats below a key
 // of value 0: without, these were lost) and are off by at most 2^-40 below.  f32 takes
-// mma.m16n8k8 on tf32 halves, x = hi + lo with hi rounded to 11 bits: hi hi + hi lo + lo hi drops lo
-// lo, 2^-22 of the product.  The tensor core cuts its f32 sums
-// instead of rounding them, so f32 sums over the keys are kept outside it: with
-// them inside, results over 2400 keys were 1.7e-6 off instead of 4.7e-7.
+// mma.m16n8k8 on tf32 halves, x = hi + lo with hi rounded to 11 bits: hi hi + hi lo +
+// lo hi drops lo lo, 2^-22 of the product.  The tensor core cuts its f32 sums instead
+// of rounding them, so f32 sums over the keys are kept outside it: with them inside,
+// results over 2400 keys were 1.7e-6 off instead of 4.7e-7.
 //
 // Work is split over a cluster of up to 16 CTAs per tile, whose partial results
 // meet in distributed shared memory: each CTA joins a slice of the output, in
@@ -45,7 +45,7 @@ constexpr int kKeys = 16;
 
 // The ring of a warp holds units of one block's K or V rows, in turn; 4 warps.
 // With 8 rows three CTAs share an SM, so that one's start and end lie under the
-// others' copies (96 ragged f16 sequences 417 us with two CTAs of 6 units a warp,
+// others' copies (in a CUDA graph, 96 ragged f16 sequences 417 us with two CTAs of 6 units a warp,
 // 402 us with three of 4; eight f32 streams 43 us with two of 3, 38 us with three of
 // 2); with more rows the registers allow two.
 template <class T, int HD, int NT>

@@ -29,9 +29,10 @@
 // product and takes 48, so that a block's products are 2560 cycles at D = 128.
 // Measured: 3200 to 3400 cycles per block of 128 keys and pair of tiles, of which
 // a softmax step's exponentials are 590 alone and 1040 beside the other tile's;
-// 9000 cycles before a CTA's first scores and 5000 after its last products.  Two
-// 2048-token chunks over 24 k and 32 k tokens (window 8192, 551 GFLOP) 487 us, 1.13
-// PFLOP/s; six prompts of 300 to 2500 tokens (151 GFLOP) 202 us.
+// 9000 cycles before a CTA's first scores and 5000 after its last products.  In a CUDA
+// graph two 2048-token chunks over 24 k and 32 k tokens (window 8192, 551 GFLOP) take
+// 499 us, 1.10 PFLOP/s (a call among others 582: the card's power bounds it), and six
+// prompts of 300 to 2500 tokens (151 GFLOP) 203 us.
 //
 // Measured and not kept: 1 to 3 of 8 pairs of exponentials as polynomials on the
 // FMA pipe (2 % faster to 5 % slower at D = 64, up to 8 % slower at 128); one score
@@ -49,7 +50,8 @@
 // nearly all of the weight, whose own value may be 0) m moves down to that step's
 // maximum.  What is still rounded more coarsely is a key beside one that is over 2^22
 // times its weight in the same 64: by up to 2^-33 of that one's.  (The long chunk
-// takes 503 us in a CUDA graph, 497 without the step down, which loses 18 nats.)
+// takes 499 us in a CUDA graph, 496 without the step down, which loses keys 18 nats
+// below a sink.)
 #include <cuda.h>
 
 #include <type_traits>
