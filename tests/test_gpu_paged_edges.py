@@ -367,3 +367,16 @@ def test_scores_that_fall_again_and_again(V, step):
     c.v[0][:64] = 0.0
     store(c)
     check_dominated(c, c.run())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q_len", [1, 90])
+def test_the_stride_of_a_single_page_says_nothing(V, dtype, q_len):
+    c = Case(V, torch, dtype, 8, 2, 64, 128, (q_len,), (100,), seed=47)
+    only = int(c.table[0, 0])
+    cache = V.PagedKvCache(c.kp[only:only + 1], c.vp[only:only + 1])
+    batch = V.PagedBatch(c.q_start, c.kv, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), c.tokens, q_len)
+    for stride in (0, 8, 1 << 40):
+        cache.desc.page_stride = stride
+        c.check(V.paged_attention(cache, batch, c.q))
+        batch.check()
